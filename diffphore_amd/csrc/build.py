@@ -92,5 +92,34 @@ def build(force=False, verbose=True):
     return OUT
 
 
+# ---- the training operators: a library of their own (include/train/diffphore_train.h), so that the hash above and what is keyed to it stay with the
+# sampling path.  Packed fp32 instructions are switched off for it: some of their forms have given wrong results on this chip.
+TRAIN = os.path.join(HERE, "train")
+TRAIN_OUT = os.path.join(TRAIN, "libdiffphore_train.so")
+TRAIN_FLAGS = FLAGS + ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+
+def build_train(force=False, verbose=True):
+    procs, objs = [], []
+    for s in sorted(glob.glob(os.path.join(TRAIN, "*.hip"))):
+        o = s[:-4] + ".o"
+        objs.append(o)
+        if force or not os.path.exists(o) or os.path.getmtime(o) < max(os.path.getmtime(d) for d in _deps(s)):
+            cmd = [HIPCC] + TRAIN_FLAGS + ["-c", s, "-o", o]
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            procs.append((s, subprocess.Popen(cmd)))
+    for s, p in procs:
+        if p.wait() != 0:
+            raise RuntimeError(f"hipcc failed on {s}")
+    if procs or not os.path.exists(TRAIN_OUT) or os.path.getmtime(TRAIN_OUT) < max(os.path.getmtime(o) for o in objs):
+        cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-Wl,--version-script=" + os.path.join(TRAIN, "exports.map")] + objs + ["-o", TRAIN_OUT]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.check_call(cmd)
+    return TRAIN_OUT
+
+
 if __name__ == "__main__":
     build(force="--force" in sys.argv)
+    build_train(force="--force" in sys.argv)

@@ -1,0 +1,122 @@
+// dpt_attn.hip - C entry points of the attention operators: checks, workspace, choice of the row blocks (kernels: dpt_attn_impl.h).
+#include "dpt_attn.h"
+
+namespace dptat {
+
+constexpr int CUS = 256;
+constexpr size_t ALIGN = 256;
+size_t up(size_t n) { return (n + ALIGN - 1) / ALIGN * ALIGN; }
+
+int check(const DptAttnArgs* a) {
+  if (!a || (a->type != DPT_F32 && a->type != DPT_BF16)) return DPT_E_BADARG;
+  if (a->B < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->dim < 1 || !(a->scale > 0.f) || a->scale > 3.4e38f) return DPT_E_BADARG;
+  if (a->n_q < 0 || a->n_k < 0 || a->max_nq < 0 || a->max_nk < 0 || a->max_nq > a->n_q || a->max_nk > a->n_k || a->n_pairs < 0 || a->splits < 0) return DPT_E_BADARG;
+  if (a->dim > 128) return DPT_E_TOOLARGE;
+  const int64_t group = a->heads / a->kv_heads, rows = (int64_t)a->max_nq * group;
+  // 32-bit row numbers, and their division by a multiplication; 32-bit workgroup numbers (32 rows or keys each at the least, 64 splits at the most)
+  if (rows * group >= (int64_t)1 << 31 || (rows / 32 + 1) * a->B * a->kv_heads * 64 >= (int64_t)1 << 31 ||
+      ((int64_t)a->max_nk / 32 + 1) * a->B * a->kv_heads >= (int64_t)1 << 31) return DPT_E_TOOLARGE;
+  return DPT_OK;
+}
+
+// Row blocks of 32 (one wave) where the largest complex has few rows: a block of 128 would leave waves without rows; otherwise 128.
+bool small_rows(const DptAttnArgs* a) { return (int64_t)a->max_nq * (a->heads / a->kv_heads) <= 64; }
+
+int splits_of(const DptAttnArgs* a) {
+  if (a->splits) return a->splits > 64 ? 64 : a->splits;
+  const int bm = small_rows(a) ? 32 : 128;
+  const int64_t rows = (int64_t)a->max_nq * (a->heads / a->kv_heads), blocks = (rows + bm - 1) / bm * a->B * a->kv_heads;
+  if (blocks == 0 || a->max_nk <= 256) return 1;
+  // enough workgroups for the chip, ranges of 128 keys at the least
+  const int64_t want = (small_rows(a) ? 4 * CUS : CUS) / blocks, most = a->max_nk / 128;
+  const int64_t s = want < most ? want : most;
+  return s < 2 ? 1 : s > 64 ? 64 : (int)s;
+}
+
+struct Ws { size_t delta, part_o, part_ml, total; };
+Ws layout(const DptAttnArgs* a, bool backward, int splits) {
+  Ws w{};
+  const size_t plane = (size_t)a->heads * a->n_q * sizeof(float);
+  if (backward) {
+    w.total = up(plane);
+  } else if (splits > 1) {
+    w.part_ml = up(plane * a->dim * splits);
+    w.total = w.part_ml + up(2 * plane * splits);
+  }
+  return w;
+}
+
+// 16-byte reads of rows of q, k, v, dout and out, 16- or 8-byte stores: the row length, every stride and every address have to allow them
+bool vec(const DptAttnArgs* a, bool backward) {
+  const int n = a->type == DPT_F32 ? 4 : 8, size = 16 / n;
+  auto ok = [&](const void* p, int64_t r, int64_t h) { return (uintptr_t)p % 16 == 0 && r % n == 0 && h % n == 0; };
+  (void)size;
+  bool v = a->dim % n == 0 && ok(a->q, a->q_row, a->q_head) && ok(a->k, a->k_row, a->k_head) && ok(a->v, a->v_row, a->v_head) && ok(a->out, 0, 0);
+  if (backward) v = v && ok(a->dout, a->dout_row, a->dout_head) && ok(a->dq, 0, 0) && ok(a->dk, 0, 0) && ok(a->dv, 0, 0);
+  return v;
+}
+
+Dev dev(const DptAttnArgs* a, bool backward) {
+  Dev d{};
+  d.a = *a;
+  d.group = a->heads / a->kv_heads;
+  d.magic = d.group > 1 ? (uint32_t)((((uint64_t)1 << 32) + d.group - 1) / d.group) : 0;
+  d.vec = vec(a, backward);
+  d.splits = 1;
+  return d;
+}
+
+bool strides_bad(const DptAttnArgs* a) {
+  return a->q_row < 0 || a->q_head < 0 || a->k_row < 0 || a->k_head < 0 || a->v_row < 0 || a->v_head < 0 || a->bias_head < 0 || a->bias_pair < 0;
+}
+
+}  // namespace dptat
+
+extern "C" {
+
+int dpt_abi_version(void) { return DPT_ABI_VERSION; }
+
+int dpt_struct_sizes(int32_t* out, int32_t n) {
+  const int32_t s[2] = {(int32_t)sizeof(DptAttnArgs), (int32_t)sizeof(DptAdamWArgs)};
+  for (int i = 0; out && i < n && i < 2; ++i) out[i] = s[i];
+  return 2;
+}
+
+size_t dpt_attn_ws_bytes(const DptAttnArgs* a, int32_t backward) {
+  if (dptat::check(a) != DPT_OK) return 0;
+  return dptat::layout(a, backward != 0, dptat::splits_of(a)).total;
+}
+
+int dpt_attn_fwd(const DptAttnArgs* a, void* stream) {
+  const int rc = dptat::check(a);
+  if (rc) return rc;
+  if (a->B == 0 || a->n_q == 0) return DPT_OK;
+  if (!a->q || !a->out || !a->stats || !a->q_ptr || !a->k_ptr || !a->pair_ptr || !a->order || (a->n_k > 0 && (!a->k || !a->v)) || dptat::strides_bad(a)) return DPT_E_BADARG;
+  dptat::Dev d = dptat::dev(a, false);
+  d.splits = dptat::splits_of(a);
+  const dptat::Ws w = dptat::layout(a, false, d.splits);
+  if (w.total && (!a->ws || a->ws_bytes < w.total || (uintptr_t)a->ws % 16)) return DPT_E_BADARG;
+  d.part_o = (float*)a->ws;
+  d.part_ml = (float*)((char*)a->ws + w.part_ml);
+  const bool small = dptat::small_rows(a);
+  const int bm = small ? 32 : 128;
+  d.tiles = (int)(((int64_t)a->max_nq * d.group + bm - 1) / bm);
+  return (int)(a->type == DPT_F32 ? dptat::fwd_f32(d, small, (hipStream_t)stream) : dptat::fwd_bf16(d, small, (hipStream_t)stream));
+}
+
+int dpt_attn_bwd(const DptAttnArgs* a, void* stream) {
+  const int rc = dptat::check(a);
+  if (rc) return rc;
+  if (a->B == 0 || (a->n_q == 0 && a->n_k == 0)) return DPT_OK;
+  if (!a->q_ptr || !a->k_ptr || !a->pair_ptr || !a->order || dptat::strides_bad(a) || a->dout_row < 0 || a->dout_head < 0) return DPT_E_BADARG;
+  if (a->n_q > 0 && (!a->q || !a->out || !a->stats || !a->dout || !a->dq)) return DPT_E_BADARG;
+  if (a->n_k > 0 && (!a->k || !a->v || !a->dk || !a->dv)) return DPT_E_BADARG;
+  const dptat::Ws w = dptat::layout(a, true, 1);
+  if (w.total && (!a->ws || a->ws_bytes < w.total || (uintptr_t)a->ws % 16)) return DPT_E_BADARG;
+  dptat::Dev d = dptat::dev(a, true);
+  d.delta = (float*)a->ws;
+  const bool sr = dptat::small_rows(a), sk = a->max_nk <= 64;
+  return (int)(a->type == DPT_F32 ? dptat::bwd_f32(d, sr, sk, (hipStream_t)stream) : dptat::bwd_bf16(d, sr, sk, (hipStream_t)stream));
+}
+
+}  // extern "C"

@@ -133,3 +133,13 @@ def clean_state_dict(state_dict: Dict[str, torch.Tensor]) -> "OrderedDict[str, t
         if tuple(out[k].shape) != tuple(want[k].shape):
             raise ValueError(f"shape mismatch for {k}: got {tuple(out[k].shape)}, want {tuple(want[k].shape)}")
     return OrderedDict((k, out[k]) for k in want)
+
+
+_BUFFERS = (".running_mean", ".running_var", ".offset")      # BatchNorm statistics, Gaussian centres: not trained
+
+
+def trainable_parameters(state_dict: Dict[str, torch.Tensor], device="cuda") -> "OrderedDict[str, torch.Tensor]":
+    """The entries of a state dict that training changes, as fp32 leaf tensors on `device` (src/utils/utils.py: the optimizer's parameter list): what
+    `optim.AdamW` takes.  `{**state_dict, **named}` is a state dict again."""
+    sd = clean_state_dict(state_dict)
+    return OrderedDict((k, v.to(device, copy=True).contiguous().requires_grad_()) for k, v in sd.items() if not k.endswith(_BUFFERS))

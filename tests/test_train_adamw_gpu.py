@@ -1,0 +1,197 @@
+"""AdamW over many tensors against the formula in 64 bits (bounds: tests/train_ref.py); 8-bit codes have to be the nearest ones exactly."""
+import pytest
+import torch
+
+import train_ref as R
+from diffphore_amd import optim
+
+pytestmark = pytest.mark.gpu
+T = {"f32": torch.float32, "bf16": torch.bfloat16}
+SIZES = [(3,), (256,), (0,), (20, 20), (1,), (7, 61), (513,), (1000, 40)]
+LR, B1, B2, EPS, WD, D = 1e-2, 0.9, 0.99, 1e-8, 0.1, 0.95
+
+
+def _setup(dtype, bits, ema, grad_dtype=None, sizes=SIZES, seed=0, **kw):
+    g = torch.Generator().manual_seed(seed)
+    params = [torch.randn(s, generator=g).to(T[dtype]).cuda() for s in sizes]
+    opt = optim.AdamW(params, lr=LR, betas=(B1, B2), eps=EPS, weight_decay=WD, no_decay=[0, 4], state_bits=bits, ema_decay=D if ema else None, **kw)
+
+    def grads(scale=1.0):
+        return [(torch.randn(s, generator=g) * scale * 10.0 ** (i % 4 - 2)).to(grad_dtype or T[dtype]).cuda() for i, s in enumerate(sizes)]
+    return params, opt, grads
+
+
+def _cut(opt, flat):
+    return [x.detach().double().cpu().reshape(-1) for x in opt.views(flat)]
+
+
+@pytest.mark.parametrize("ema", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype, grad_dtype", [("f32", None), ("bf16", None), ("bf16", torch.float32)])
+def test_steps_match_the_formula(dtype, grad_dtype, bits, ema):
+    params, opt, grads = _setup(dtype, bits, ema, grad_dtype)
+    for t in range(1, 5):
+        before = [x.double().cpu().reshape(-1) for x in (opt.views(opt.master) if dtype == "bf16" else [p.clone() for p in params])]
+        m0, v0 = (_cut(opt, f.clone()) for f in opt.moments())
+        codes0 = (opt.exp_avg.cpu(), opt.exp_avg_scale.cpu(), opt.exp_avg_sq.cpu(), opt.exp_avg_sq_scale.cpu()) if bits == 8 else None
+        e0 = _cut(opt, opt.ema.clone()) if ema else None
+        if bits == 8:                            # what the codes stand for, in 64 bits
+            exact = [R.decode(codes0[0], codes0[1], 2), R.decode(codes0[2], codes0[3], 4)]
+            m0, v0 = ([f[b * 256:b * 256 + n] for b, n in zip(opt.first_block, opt._numel)] for f in exact)
+        gs = grads()
+        opt.step(gs)
+        m1, v1 = (_cut(opt, f) for f in opt.moments())
+        for i, p in enumerate(params):
+            g = gs[i].double().cpu().reshape(-1)
+            (pr, bp), (mr, bm), (vr, bv) = R.adamw(before[i], g, m0[i], v0[i], t, LR, B1, B2, EPS, 0.0 if i in (0, 4) else WD)
+            new = (opt.views(opt.master)[i] if dtype == "bf16" else p).double().cpu().reshape(-1)
+            R.within(new, pr, bp, f"p{i} step {t}")
+            if dtype == "bf16":
+                assert torch.equal(p.reshape(-1), opt.views(opt.master)[i].bfloat16().reshape(-1))
+            if ema:
+                R.within(opt.views(opt.ema)[i].reshape(-1), D * e0[i] + (1 - D) * new, 4 * R.F32 * (e0[i].abs() + new.abs()), "ema")
+            if bits == 32:
+                R.within(m1[i], mr, bm, "m")
+                R.within(v1[i], vr, bv, "v")
+            else:
+                pad = -len(mr) % 256
+                for x, power, code, scale in ((mr, 2, opt.exp_avg, opt.exp_avg_scale), (vr, 4, opt.exp_avg_sq, opt.exp_avg_sq_scale)):
+                    if not len(x):
+                        continue
+                    c, s = R.encode(torch.nn.functional.pad(x, (0, pad)), power)
+                    lo, hi = opt.first_block[i], opt.first_block[i + 1]
+                    assert torch.equal(code[lo * 256:hi * 256].cpu(), c), f"codes of power {power}, tensor {i}, step {t}"
+                    # the scale is the 64-bit maximum rounded once: an ulp where the kernel's 64-bit sum differs in its last bit
+                    assert torch.allclose(scale[lo:hi].cpu(), s, rtol=2.0 ** -23, atol=0)
+    assert opt.state_dict()["step"] == 4
+
+
+def test_many_tensors_take_several_launches():
+    sizes = [(i % 5 + 1,) for i in range(900)]
+    params, opt, grads = _setup("f32", 32, True, sizes=sizes)
+    one, opt1, grads1 = _setup("f32", 32, True, sizes=sizes)
+    gs = grads()
+    flat = torch.cat([g.reshape(-1) for g in gs])
+    opt.step(gs)
+    single = optim.AdamW([torch.cat([p.reshape(-1) for p in one])], lr=LR, betas=(B1, B2), eps=EPS, weight_decay=0.0)
+    single.step([flat])
+    no_wd = optim.AdamW(one, lr=LR, betas=(B1, B2), eps=EPS, weight_decay=0.0)
+    no_wd.step(gs)
+    assert torch.equal(torch.cat([p.reshape(-1) for p in one]), single.params[0])
+    assert opt.state_dict()["step"] == no_wd.state_dict()["step"] == 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_views_at_odd_addresses_and_padding(bits):
+    """parameters and gradients that start off a 16-byte border; nothing beside them is written; the padding of the state stays 0"""
+    base = torch.randn(4000, device="cuda")
+    gbase = torch.randn(4000, device="cuda")
+    cuts = [(1, 1000), (1003, 259), (1263, 512), (1777, 2000)]
+    copy = base.clone()
+    params = [base[a:a + n] for a, n in cuts]
+    plain = [copy[a:a + n].clone() for a, n in cuts]
+    opt, ref = (optim.AdamW(p, lr=LR, betas=(B1, B2), weight_decay=WD, state_bits=bits) for p in (params, plain))
+    for _ in range(3):
+        gbase = torch.randn(4000, device="cuda")
+        opt.step([gbase[a:a + n] for a, n in cuts])
+        ref.step([gbase[a:a + n].clone() for a, n in cuts])
+    assert all(torch.equal(p, r) for p, r in zip(params, plain))
+    inside = torch.zeros(4000, dtype=torch.bool)
+    for a, n in cuts:
+        inside[a:a + n] = True
+    assert torch.equal(base.cpu()[~inside], copy.cpu()[~inside])
+    m, v = opt.moments()
+    for a, b, n in zip(opt.first_block, opt.first_block[1:], opt._numel):
+        assert not m[a * 256 + n:b * 256].any() and not v[a * 256 + n:b * 256].any()
+
+
+def test_none_gradients_grad_scale_lr_and_dicts():
+    p = {"a": torch.ones(300, device="cuda"), "b": torch.ones(5, device="cuda"), "c": torch.ones(2, 2, device="cuda")}
+    opt = optim.AdamW(p, lr=0.5, weight_decay=0.0, no_decay=["b"], ema_decay=0.0)
+    opt.step({"a": torch.full((300,), 2.0, device="cuda"), "c": torch.ones(2, 2, device="cuda")}, lr=torch.tensor(0.25, device="cuda"),
+             grad_scale=torch.tensor(0.5, device="cuda"))
+    assert torch.equal(p["b"], torch.ones(5, device="cuda")) and not opt.views(opt.exp_avg)["b"].any()
+    # the first step moves every entry by lr (m / c1) / sqrt(v / c2) = lr
+    assert torch.allclose(p["a"], torch.full_like(p["a"], 0.75), atol=1e-5) and torch.allclose(p["c"], torch.full_like(p["c"], 0.75), atol=1e-5)
+    assert torch.allclose(opt.views(opt.exp_avg)["a"], torch.full((300,), 0.1, device="cuda"))
+    assert torch.equal(opt.ema_parameters()["a"], p["a"])
+    for q in p.values():
+        q.requires_grad_()
+    (p["a"].sum() * 3).backward()
+    opt.step()                                   # .grad, and None for the others
+    opt.zero_grad()
+    assert p["a"].grad is None and opt.state_dict()["step"] == 2
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_dict_round_trip(bits):
+    params, opt, grads = _setup("bf16", bits, True)
+    for _ in range(3):
+        opt.step(grads())
+    clones = [p.clone() for p in params]
+    again = optim.AdamW(clones, lr=LR, betas=(B1, B2), eps=EPS, weight_decay=WD, no_decay=[0, 4], state_bits=bits, ema_decay=D)
+    again.load_state_dict(opt.state_dict())
+    g = grads()
+    opt.step(g)
+    again.step(g)
+    assert all(torch.equal(a, b) for a, b in zip(params, clones)) and torch.equal(opt.exp_avg, again.exp_avg) and torch.equal(opt.ema, again.ema)
+    wrong = optim.AdamW(clones, state_bits=40 - bits, ema_decay=D)
+    with pytest.raises(ValueError):
+        wrong.load_state_dict(opt.state_dict())
+    with pytest.raises(ValueError):
+        optim.AdamW(clones, state_bits=bits).load_state_dict(opt.state_dict())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_gradients_that_are_not_finite_and_extreme_sizes(bits):
+    p = torch.ones(1024, device="cuda")
+    opt = optim.AdamW([p], lr=1e-3, weight_decay=0.0, state_bits=bits)
+    g = torch.zeros(1024, device="cuda")
+    g[300], g[600] = float("nan"), 1e-30
+    g[700:720] = torch.logspace(-18, 15, 20, device="cuda")
+    opt.step([g])
+    m, v = opt.moments()
+    bad = torch.isnan(p)
+    assert bad[300] and bad.sum() == 1
+    where = torch.zeros(1024, dtype=torch.bool, device="cuda")
+    where[300 if bits == 32 else slice(256, 512)] = True
+    assert torch.equal(torch.isnan(m), where) and torch.equal(torch.isnan(v), where)
+    if bits == 8:
+        assert opt.exp_avg_sq[700:720].min() >= 1                       # never 0 for a positive second moment
+    opt.step([torch.zeros(1024, device="cuda")])
+    assert torch.isnan(p[256:512]).any() and torch.isfinite(p[512:]).all() and torch.isfinite(p[:256]).all()
+
+
+def test_eight_bits_move_parameters_as_32_do():
+    """400 steps on a quadratic from one start: the 8-bit run stays within a tenth of the way that the parameters travel"""
+    g = torch.Generator().manual_seed(2)
+    start, goal = torch.randn(2000, generator=g).cuda(), torch.randn(2000, generator=g).cuda()
+    ends = []
+    for bits in (32, 8):
+        p = start.clone()
+        opt = optim.AdamW([p], lr=3e-3, weight_decay=0.0, state_bits=bits)
+        for _ in range(400):
+            opt.step([p - goal])
+        ends.append(p)
+    assert (ends[0] - ends[1]).norm() < 0.1 * (ends[0] - start).norm()
+
+
+def test_refusals():
+    a = torch.ones(8, device="cuda")
+    for params in ([a.half()], [a, a.bfloat16()], [a, a], [a, a[4:]], [torch.ones(4, 4, device="cuda").t()], [a.cpu()], []):
+        with pytest.raises((TypeError, ValueError)):
+            optim.AdamW(params)
+    for kw in (dict(lr=-1.0), dict(eps=-1.0), dict(betas=(1.0, 0.9)), dict(weight_decay=-1.0), dict(state_bits=16), dict(ema_decay=1.5), dict(no_decay=[1]),
+               dict(lr=float("nan"))):
+        with pytest.raises(ValueError):
+            optim.AdamW([a], **kw)
+    opt = optim.AdamW([a])
+    for g in ([], [a, a], [a.half()], [a.bfloat16()], [a[:4]], [torch.ones(16, device="cuda")[::2]], [a.cpu()], {"x": a}):
+        with pytest.raises((TypeError, ValueError)):
+            opt.step(g)
+    for kw in (dict(lr=torch.tensor(0.1)), dict(lr=torch.ones(2, device="cuda")), dict(grad_scale=torch.ones(1, device="cuda").double())):
+        with pytest.raises(ValueError):
+            opt.step([torch.zeros(8, device="cuda")], **kw)
+    with pytest.raises(ValueError):
+        opt.ema_parameters()
+    assert torch.equal(a, torch.ones(8, device="cuda"))
