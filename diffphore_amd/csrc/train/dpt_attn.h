@@ -24,7 +24,7 @@ struct Dev {                     // DptAttnArgs plus what every workgroup would 
   uint32_t magic;                // r / group = mulhi(r, magic) for group > 1
   int tiles;                     // row (backward: key) blocks of the largest complex
   int vec;                       // rows of q, k, v, dout may be read, out and gradients written, 16 bytes at a time
-  float* delta;                  // [heads, n_q] sum_d dout out (backward)
+  float *delta, *fac0, *fac1;    // backward, [heads, n_q] each: sum_d dout out; what turns a score into a probability (Probs)
   float *part_o, *part_ml;       // forward with splits: [splits, n_q, heads, dim] and [splits, 2, heads, n_q]
 };
 
@@ -131,6 +131,7 @@ __device__ __forceinline__ void cols_times(const float* tile, int row0, int lane
   }
 }
 
+// over a lane pair (l, l + 32)
 __device__ __forceinline__ float half_max(float x) { return fmaxf(x, __shfl_xor(x, 32, 64)); }
 __device__ __forceinline__ float half_sum(float x) { return x + __shfl_xor(x, 32, 64); }
 
@@ -155,15 +156,38 @@ __device__ __forceinline__ void store_col(T* __restrict__ row, int h, int dim, i
     }
 }
 
-// rows [first, first + ROWS) of a complex's keys (or values) into a tile; rows from `limit` on repeat the last one (their scores are masked: repeating
-// a row that is there brings in no value that the result does not hold anyway)
+// A tile of ROWS rows is filled by the workgroup's NT lanes, 16 bytes per lane and turn, in LDS order: turn n of lane t fills chunk n NT + t, so the
+// lane's source is the chunk that the permutation puts there.  `at(row)` gives a row's address.
+//   vec: straight into LDS (no registers; the tile is there after the next __syncthreads, which waits for memory).  Chunks behind dim are not
+//        fetched: they hold the zeros that zero_pad() put there before the loop.
+//   otherwise: through registers, element by element.
+template <typename T, int DP, int ROWS, int NT, typename At>
+__device__ __forceinline__ void stage(T* tile, int dim, int vec, At at) {
+  constexpr int N = NC<T, DP>, CH = Tr<T>::CH, TURNS = ROWS * N / NT;
+  static_assert(ROWS * N % NT == 0, "every lane in every turn");
+#pragma unroll
+  for (int n = 0; n < TURNS; ++n) {
+    const int i = n * NT + threadIdx.x, row = i / N, c = (i % N) ^ sw<N>(row);
+    if (vec) {
+      T* dst = tile + (n * NT + __builtin_amdgcn_readfirstlane(threadIdx.x & ~63)) * CH;
+      if (c * CH < dim)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(at(row) + c * CH),
+                                         (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+    } else {
+      *reinterpret_cast<typename Tr<T>::frag*>(tile + i * CH) = load_chunk<T>(at(row), c, dim, 0);
+    }
+  }
+}
 template <typename T, int DP, int ROWS, int NT>
-__device__ __forceinline__ void stage_keys(T* tile, const T* __restrict__ base, int64_t stride, int first, int limit, int dim, int vec) {
-  constexpr int N = NC<T, DP>;
-#pragma unroll 4
+__device__ __forceinline__ void zero_pad(T* tile, int dim) {
+  constexpr int N = NC<T, DP>, CH = Tr<T>::CH;
+  if (dim == DP) return;
   for (int i = threadIdx.x; i < ROWS * N; i += NT) {
-    const int row = i / N, c = i % N, at = first + row < limit ? first + row : limit - 1;
-    *reinterpret_cast<typename Tr<T>::frag*>(tile + (row * N + (c ^ sw<N>(row))) * Tr<T>::CH) = load_chunk<T>(base + at * stride, c, dim, vec);
+    const int row = i / N, c = (i % N) ^ sw<N>(row);
+    typename Tr<T>::frag z;
+#pragma unroll
+    for (int e = 0; e < CH; ++e) z[e] = (T)0.f;
+    if (c * CH >= dim) *reinterpret_cast<typename Tr<T>::frag*>(tile + i * CH) = z;
   }
 }
 

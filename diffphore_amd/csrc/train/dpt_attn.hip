@@ -38,7 +38,8 @@ Ws layout(const DptAttnArgs* a, bool backward, int splits) {
   Ws w{};
   const size_t plane = (size_t)a->heads * a->n_q * sizeof(float);
   if (backward) {
-    w.total = up(plane);
+    w.delta = up(plane);                 // one of three planes
+    w.total = 3 * w.delta;
   } else if (splits > 1) {
     w.part_ml = up(plane * a->dim * splits);
     w.total = w.part_ml + up(2 * plane * splits);
@@ -115,6 +116,8 @@ int dpt_attn_bwd(const DptAttnArgs* a, void* stream) {
   if (w.total && (!a->ws || a->ws_bytes < w.total || (uintptr_t)a->ws % 16)) return DPT_E_BADARG;
   dptat::Dev d = dptat::dev(a, true);
   d.delta = (float*)a->ws;
+  d.fac0 = (float*)((char*)a->ws + w.delta);
+  d.fac1 = (float*)((char*)a->ws + 2 * w.delta);
   const bool sr = dptat::small_rows(a), sk = a->max_nk <= 64;
   return (int)(a->type == DPT_F32 ? dptat::bwd_f32(d, sr, sk, (hipStream_t)stream) : dptat::bwd_bf16(d, sr, sk, (hipStream_t)stream));
 }

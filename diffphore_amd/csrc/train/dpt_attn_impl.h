@@ -41,45 +41,91 @@ __device__ __forceinline__ Row row_at(const Dev& d, const Place& p, int r) {
   return x;
 }
 
-// scores of 32 keys x the lane's row: scaled, biased, masked.  key0: the tile's first key; lim: keys that the row sees
+// From a product q.k to exp(s - m).  FAST (bf16 without a bias): scores stay unscaled, exp2(fma(x, scale log2 e, -m scale log2 e)) - one operation and the
+// exponential, an error of a few 2^-24 |m|, far below the rounding of a bf16 probability.  Otherwise exp2((s - m) log2 e) with the difference first:
+// a row of the type's lowest values is then a row of exact zeros under the exponential, and fp32 keeps its last bits.
+template <typename T, bool BIAS> constexpr bool FAST = sizeof(T) == 2 && !BIAS;
+
+// scores of 32 keys x the lane's row: scaled and biased unless FAST, masked.  key0: the tile's first key; lim: keys that the row sees; part: some
+// row of the wave sees only a part of the tile
 template <typename T, bool BIAS>
 __device__ __forceinline__ void finish_scores(const Dev& d, f16v& s, int key0, int h, int lim, bool part, const T* __restrict__ bias) {
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
     const int key = key0 + 8 * (e >> 2) + 4 * h + (e & 3);
-    float x = s[e] * d.a.scale;
     if constexpr (BIAS) {
-      const float bv = key < lim ? (float)bias[key * d.a.bias_pair] : NEG_INF;
-      x = bv == NEG_INF ? NEG_INF : x + bv;
-    } else {
-      if (part) x = key < lim ? x : NEG_INF;
+      const float x = s[e] * d.a.scale, bv = key < lim ? (float)bias[key * d.a.bias_pair] : NEG_INF;
+      s[e] = bv == NEG_INF ? NEG_INF : x + bv;
+    } else if constexpr (!FAST<T, BIAS>) {
+      s[e] *= d.a.scale;
     }
-    s[e] = x;
+  }
+  if constexpr (!BIAS) {
+    if (part) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = key0 + 8 * (e >> 2) + 4 * h + (e & 3) < lim ? s[e] : NEG_INF;
+    }
   }
 }
 
+// a row block's view of its keys, common to the forward and the dq kernel
+template <int BM>
+struct RowBlock {
+  Row row;
+  bool live;
+  int lim, lim_lo, lim_hi, last;   // keys that the lane's row, the wave's first and last row, the block's last row see
+  __device__ __forceinline__ RowBlock(const Dev& d, const Place& p, int tile, int lane) {
+    const int w0 = tile * BM + (threadIdx.x & ~63) / 2, r = w0 + (lane & 31), end = p.rows - 1;
+    live = r <= end;
+    row = row_at(d, p, min(r, end));
+    lim = keys_seen(d, p, row.i);
+    lim_lo = __builtin_amdgcn_readfirstlane(keys_seen(d, p, div_group(d, min(w0, end))));
+    lim_hi = __builtin_amdgcn_readfirstlane(keys_seen(d, p, div_group(d, min(w0 + 31, end))));
+    last = keys_seen(d, p, div_group(d, min(tile * BM + BM - 1, end)));
+  }
+};
+
+template <int N>
+__device__ __forceinline__ void zero(f16v* x) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[i][e] = 0.f;
+}
+
 // ---- forward -----------------------------------------------------------------------------------------------------------------------------------
-// NW waves x 32 rows; keys in tiles of BN.  Running maximum and sum per row, one pass over the keys.
+// NW waves x 32 rows; keys in tiles of BN, the next tile on its way into the other LDS buffer while one is worked on.  One pass over the keys with a
+// running base and sum per row.  The base follows the row's maximum only when that has moved by more than 2^8 (exp of the difference then still has all its
+// bits, and so has a bf16 of it), so the accumulators are rescaled a few times per row instead of once per tile.
 template <typename T, int DP, int NW, int BN, bool BIAS>
 __global__ __launch_bounds__(64 * NW) void fwd_kernel(Dev d) {
-  __shared__ __attribute__((aligned(16))) T kt[BN * DP], vt[BN * DP];
-  const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5, wave = threadIdx.x / 64;
+  __shared__ __attribute__((aligned(16))) T kt0[BN * DP], vt0[BN * DP], kt1[BN * DP], vt1[BN * DP];
+  constexpr int NT = 64 * NW, BM = 32 * NW, J = BN / 32;
+  constexpr float FAR = 8.f;
+  const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
   int id = blockIdx.x, tile;
   const int split = id % d.splits;
   const Place p = place(d, id / d.splits, &tile);
-  constexpr int BM = 32 * NW;
   const int tiles = (p.rows + BM - 1) / BM;
   if (tile >= tiles) return;
   if (d.a.causal) tile = tiles - 1 - tile;                   // the longest rows first
-  const int r0 = tile * BM, r = r0 + wave * 32 + l31;
-  const Row row = row_at(d, p, r < p.rows ? r : p.rows - 1);
-  const int lim = keys_seen(d, p, row.i);
-  const int lim_lo = keys_seen(d, p, div_group(d, min(r0 + wave * 32, p.rows - 1)));
-  const int lim_hi = keys_seen(d, p, div_group(d, min(r0 + wave * 32 + 31, p.rows - 1)));
-  const int last = keys_seen(d, p, div_group(d, min(r0 + BM, p.rows) - 1));
-  const int ktiles = (last + BN - 1) / BN, per = (ktiles + d.splits - 1) / d.splits;
+  const RowBlock<BM> rb(d, p, tile, lane);
+  const Row row = rb.row;
+  const int ktiles = (rb.last + BN - 1) / BN, per = (ktiles + d.splits - 1) / d.splits;
   const int t0 = split * per, t1 = min(t0 + per, ktiles);
 
+  const T* kb = (const T*)d.a.k + (int64_t)p.k0 * d.a.k_row + p.hk * d.a.k_head;
+  const T* vb = (const T*)d.a.v + (int64_t)p.k0 * d.a.v_row + p.hk * d.a.v_head;
+  // keys from the last one on repeat it: their scores are masked, and it brings in no value that the result does not hold anyway
+  auto fetch = [&](T* kt, T* vt, int t) __attribute__((always_inline)) {
+    stage<T, DP, BN, NT>(kt, d.a.dim, d.vec, [&](int r) { return kb + (int64_t)min(t * BN + r, p.nk - 1) * d.a.k_row; });
+    stage<T, DP, BN, NT>(vt, d.a.dim, d.vec, [&](int r) { return vb + (int64_t)min(t * BN + r, p.nk - 1) * d.a.v_row; });
+  };
+  if (t0 < t1) fetch(kt0, vt0, t0);
+  zero_pad<T, DP, BN, NT>(kt0, d.a.dim);
+  zero_pad<T, DP, BN, NT>(vt0, d.a.dim);
+  zero_pad<T, DP, BN, NT>(kt1, d.a.dim);
+  zero_pad<T, DP, BN, NT>(vt1, d.a.dim);
   typename Tr<T>::frag qf[NC<T, DP> / 2];
   {
     const T* q = (const T*)d.a.q + row.token * d.a.q_row + row.head * d.a.q_head;
@@ -87,61 +133,68 @@ __global__ __launch_bounds__(64 * NW) void fwd_kernel(Dev d) {
     for (int s = 0; s < NC<T, DP> / 2; ++s) qf[s] = load_chunk<T>(q, 2 * s + h, d.a.dim, d.vec);
   }
   const T* bias = BIAS ? (const T*)d.a.bias + row.head * d.a.bias_head + (p.pair0 + (int64_t)row.i * p.nk) * d.a.bias_pair : nullptr;
-  const T* kb = (const T*)d.a.k + (int64_t)p.k0 * d.a.k_row + p.hk * d.a.k_head;
-  const T* vb = (const T*)d.a.v + (int64_t)p.k0 * d.a.v_row + p.hk * d.a.v_head;
+  const float c = FAST<T, BIAS> ? d.a.scale * LOG2E : LOG2E;   // exp(s - base) = exp2((x - base) c)
 
   f16v o[DP / 32];
-#pragma unroll
-  for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
-  float m = NEG_INF, l = 0.f;
-  for (int t = t0; t < t1; ++t) {
+  zero<DP / 32>(o);
+  float m = NEG_INF, base = NEG_INF, l = 0.f;                // of the scores as they are held; l: this half's share of the sum
+  auto work = [&](const T* kt, const T* vt, int t) __attribute__((always_inline)) {
     const int key0 = t * BN;
-    __syncthreads();
-    stage_keys<T, DP, BN, 64 * NW>(kt, kb, d.a.k_row, key0, p.nk, d.a.dim, d.vec);
-    stage_keys<T, DP, BN, 64 * NW>(vt, vb, d.a.v_row, key0, p.nk, d.a.dim, d.vec);
-    __syncthreads();
-    if (key0 >= lim_hi) continue;                            // (wave-uniform; the barriers above are still met by every wave)
-    f16v s[BN / 32];
+    if (key0 >= rb.lim_hi) return;
+    f16v s[J];
+    zero<J>(s);
+#pragma unroll
+    for (int j = 0; j < J; ++j) s[j] = rows_times<T, DP>(kt, 32 * j, l31, h, qf, s[j]);
     float top = m;
 #pragma unroll
-    for (int j = 0; j < BN / 32; ++j) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[j][e] = 0.f;
-      s[j] = rows_times<T, DP>(kt, 32 * j, l31, h, qf, s[j]);
-      finish_scores<T, BIAS>(d, s[j], key0 + 32 * j, h, lim, key0 + BN > lim_lo, bias);
+    for (int j = 0; j < J; ++j) {
+      finish_scores<T, BIAS>(d, s[j], key0 + 32 * j, h, rb.lim, key0 + BN > rb.lim_lo, bias);
 #pragma unroll
       for (int e = 0; e < 16; ++e) top = fmaxf(top, s[j][e]);
     }
-    top = half_max(top);
-    const float base = top == NEG_INF ? 0.f : top;           // nothing seen yet: exp of -inf - 0
-    const float alpha = __builtin_amdgcn_exp2f((m - base) * LOG2E);
-    float sum = 0.f;
+    m = half_max(top);
+    if (__any((m - base) * c > FAR)) {                       // (base -inf: the first keys that the row sees)
+      const float nb = fmaxf(base, m), alpha = __builtin_amdgcn_exp2f((base - (nb == NEG_INF ? 0.f : nb)) * c);
+      base = nb;
+      l *= alpha;
 #pragma unroll
-    for (int j = 0; j < BN / 32; ++j)
+      for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+    }
+    const float b0 = base == NEG_INF ? 0.f : base, nbc = -b0 * c;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        s[j][e] = __builtin_amdgcn_exp2f((s[j][e] - base) * LOG2E);
-        sum += s[j][e];
+        s[j][e] = __builtin_amdgcn_exp2f(FAST<T, BIAS> ? fmaf(s[j][e], c, nbc) : (s[j][e] - b0) * c);
+        l += s[j][e];
       }
-    l = l * alpha + half_sum(sum);
-    m = top;
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
-#pragma unroll
-    for (int j = 0; j < BN / 32; ++j) cols_times<DP>(vt, 32 * j, lane, (const float*)&s[j], o);
+    for (int j = 0; j < J; ++j) cols_times<DP>(vt, 32 * j, lane, (const float*)&s[j], o);
+  };
+  // one barrier per tile: it waits for the tile's fetch and for the last reads of the buffer that the next fetch overwrites
+  for (int t = t0; t < t1; t += 2) {
+    __syncthreads();
+    if (t + 1 < t1) fetch(kt1, vt1, t + 1);
+    work(kt0, vt0, t);
+    if (t + 1 >= t1) break;
+    __syncthreads();
+    if (t + 2 < t1) fetch(kt0, vt0, t + 2);
+    work(kt1, vt1, t + 1);
   }
-  if (r >= p.rows) return;
+  if (!rb.live) return;
+  // the sum in terms of the true maximum
+  l = half_sum(l);
+  const float lm = m == NEG_INF ? 0.f : l * __builtin_amdgcn_exp2f((base - m) * c), mm = FAST<T, BIAS> ? m * d.a.scale : m;
   const int64_t at = row.token * d.a.heads + row.head, st = (int64_t)row.head * d.a.n_q + row.token, plane = (int64_t)d.a.heads * d.a.n_q;
   if (d.splits == 1) {
     store_col<T, DP>((T*)d.a.out + at * d.a.dim, h, d.a.dim, d.vec, o, l == 0.f ? 0.f : 1.f / l);
-    if (h == 0) { d.a.stats[st] = m; d.a.stats[plane + st] = l; }
+    if (h == 0) { d.a.stats[st] = mm; d.a.stats[plane + st] = lm; }
   } else {
-    store_col<float, DP>(d.part_o + (split * plane + at) * d.a.dim, h, d.a.dim, d.a.dim % 4 == 0, o, 1.f);
-    if (h == 0) { d.part_ml[2 * split * plane + st] = m; d.part_ml[(2 * split + 1) * plane + st] = l; }
+    const float f = m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((base - m) * c);
+    store_col<float, DP>(d.part_o + (split * plane + at) * d.a.dim, h, d.a.dim, d.a.dim % 4 == 0, o, f);
+    if (h == 0) { d.part_ml[2 * split * plane + st] = mm; d.part_ml[(2 * split + 1) * plane + st] = lm; }
   }
 }
 
@@ -171,29 +224,57 @@ __global__ __launch_bounds__(256) void join_kernel(Dev d) {
 }
 
 // ---- backward: gradients of the queries and of the bias -------------------------------------------------------------------------------------------
-// As the forward pass, with the probabilities formed again from the stored statistics: ds = p (do.v - delta), dq += ds k.
-// Also writes delta = sum_d do o for the second kernel.
+// What the backward kernels make of a row's statistics.  FAST: p = exp2(fma(x, scale log2 e, f0)), f0 = -(m log2 e + log2 l) (-inf for a row that sees nothing);
+// otherwise p = exp2((s - f0) log2 e) f1 with f0 = m, f1 = 1 / l (0 and 0).
+template <typename T, bool BIAS>
+struct Probs {
+  float f0, f1;
+  __device__ __forceinline__ Probs(float m, float l) {
+    if constexpr (FAST<T, BIAS>) {
+      f0 = l == 0.f ? NEG_INF : -(m * LOG2E + __builtin_amdgcn_logf(l));
+      f1 = 0.f;
+    } else {
+      f0 = m == NEG_INF ? 0.f : m;
+      f1 = l == 0.f ? 0.f : 1.f / l;
+    }
+  }
+  static __device__ __forceinline__ float p(float x, float c, float f0, float f1) {
+    return FAST<T, BIAS> ? __builtin_amdgcn_exp2f(fmaf(x, c, f0)) : __builtin_amdgcn_exp2f((x - f0) * c) * f1;
+  }
+};
+
+// As the forward pass, with the probabilities formed again from the stored statistics: ds = p (do.v - delta), dq += ds k.  Writes delta = sum_d do o and the
+// rows' factors for the second kernel.  Where a complex's keys are one tile, delta is taken as sum_j p_j do.v_j instead: the stored out is rounded to
+// its type, and with few keys that rounding does not average out.
 template <typename T, int DP, int NW, int BN, bool BIAS>
 __global__ __launch_bounds__(64 * NW) void dq_kernel(Dev d) {
-  __shared__ __attribute__((aligned(16))) T kt[BN * DP], vt[BN * DP];
-  const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5, wave = threadIdx.x / 64;
+  __shared__ __attribute__((aligned(16))) T kt0[BN * DP], vt0[BN * DP], kt1[BN * DP], vt1[BN * DP];
+  constexpr int NT = 64 * NW, BM = 32 * NW, J = BN / 32;
+  const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
   int tile;
   const Place p = place(d, blockIdx.x, &tile);
-  constexpr int BM = 32 * NW;
   const int tiles = (p.rows + BM - 1) / BM;
   if (tile >= tiles) return;
   if (d.a.causal) tile = tiles - 1 - tile;
-  const int r0 = tile * BM, r = r0 + wave * 32 + l31;
-  const bool live = r < p.rows;
-  const Row row = row_at(d, p, live ? r : p.rows - 1);
-  const int lim = keys_seen(d, p, row.i);
-  const int lim_lo = keys_seen(d, p, div_group(d, min(r0 + wave * 32, p.rows - 1)));
-  const int lim_hi = keys_seen(d, p, div_group(d, min(r0 + wave * 32 + 31, p.rows - 1)));
-  const int last = keys_seen(d, p, div_group(d, min(r0 + BM, p.rows) - 1));
+  const RowBlock<BM> rb(d, p, tile, lane);
+  const Row row = rb.row;
   // a bias gradient is written for every pair, 0 for those behind the causal edge
-  const int end = BIAS && d.a.dbias ? p.nk : last;
+  const int ktiles = ((BIAS && d.a.dbias ? p.nk : rb.last) + BN - 1) / BN;
+
+  const T* kb = (const T*)d.a.k + (int64_t)p.k0 * d.a.k_row + p.hk * d.a.k_head;
+  const T* vb = (const T*)d.a.v + (int64_t)p.k0 * d.a.v_row + p.hk * d.a.v_head;
+  auto fetch = [&](T* kt, T* vt, int t) __attribute__((always_inline)) {
+    stage<T, DP, BN, NT>(kt, d.a.dim, d.vec, [&](int r) { return kb + (int64_t)min(t * BN + r, p.nk - 1) * d.a.k_row; });
+    stage<T, DP, BN, NT>(vt, d.a.dim, d.vec, [&](int r) { return vb + (int64_t)min(t * BN + r, p.nk - 1) * d.a.v_row; });
+  };
+  if (ktiles) fetch(kt0, vt0, 0);
+  zero_pad<T, DP, BN, NT>(kt0, d.a.dim);
+  zero_pad<T, DP, BN, NT>(vt0, d.a.dim);
+  zero_pad<T, DP, BN, NT>(kt1, d.a.dim);
+  zero_pad<T, DP, BN, NT>(vt1, d.a.dim);
 
   const int64_t at = row.token * d.a.heads + row.head, st = (int64_t)row.head * d.a.n_q + row.token, plane = (int64_t)d.a.heads * d.a.n_q;
+  const bool one = p.nk <= BN;
   typename Tr<T>::frag qf[NC<T, DP> / 2], gf[NC<T, DP> / 2];
   float delta = 0.f;
   {
@@ -204,136 +285,189 @@ __global__ __launch_bounds__(64 * NW) void dq_kernel(Dev d) {
     for (int s = 0; s < NC<T, DP> / 2; ++s) {
       qf[s] = load_chunk<T>(q, 2 * s + h, d.a.dim, d.vec);
       gf[s] = load_chunk<T>(g, 2 * s + h, d.a.dim, d.vec);
-      const typename Tr<T>::frag of = load_chunk<T>(o, 2 * s + h, d.a.dim, d.vec);
-#pragma unroll
-      for (int e = 0; e < Tr<T>::CH; ++e) delta = fmaf((float)gf[s][e], (float)of[e], delta);
     }
-    delta = half_sum(delta);
-    if (live && h == 0) d.delta[st] = delta;
+    if (!one) {
+#pragma unroll
+      for (int s = 0; s < NC<T, DP> / 2; ++s) {
+        const typename Tr<T>::frag of = load_chunk<T>(o, 2 * s + h, d.a.dim, d.vec);
+#pragma unroll
+        for (int e = 0; e < Tr<T>::CH; ++e) delta = fmaf((float)gf[s][e], (float)of[e], delta);
+      }
+      delta = half_sum(delta);
+    }
   }
-  const float m = d.a.stats[st], l = d.a.stats[plane + st];
-  const float base = m == NEG_INF ? 0.f : m, inv = l == 0.f ? 0.f : 1.f / l;
+  const Probs<T, BIAS> f(d.a.stats[st], d.a.stats[plane + st]);
+  const float c = FAST<T, BIAS> ? d.a.scale * LOG2E : LOG2E;
   const T* bias = BIAS ? (const T*)d.a.bias + row.head * d.a.bias_head + (p.pair0 + (int64_t)row.i * p.nk) * d.a.bias_pair : nullptr;
   T* dbias = BIAS && d.a.dbias ? (T*)d.a.dbias + row.head * d.a.n_pairs + p.pair0 + (int64_t)row.i * p.nk : nullptr;
-  const T* kb = (const T*)d.a.k + (int64_t)p.k0 * d.a.k_row + p.hk * d.a.k_head;
-  const T* vb = (const T*)d.a.v + (int64_t)p.k0 * d.a.v_row + p.hk * d.a.v_head;
 
   f16v dq[DP / 32];
+  zero<DP / 32>(dq);
+  auto work = [&](const T* kt, const T* vt, int t) __attribute__((always_inline)) {
+    const int key0 = t * BN;
+    if (key0 >= rb.lim_hi && !dbias) return;
+    const bool part = key0 + BN > rb.lim_lo;
+    f16v s[J], g[J];
+    zero<J>(s);
+    zero<J>(g);
 #pragma unroll
-  for (int i = 0; i < DP / 32; ++i)
+    for (int j = 0; j < J; ++j) s[j] = rows_times<T, DP>(kt, 32 * j, l31, h, qf, s[j]);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) dq[i][e] = 0.f;
-  for (int key0 = 0; key0 < end; key0 += BN) {
-    __syncthreads();
-    stage_keys<T, DP, BN, 64 * NW>(kt, kb, d.a.k_row, key0, p.nk, d.a.dim, d.vec);
-    stage_keys<T, DP, BN, 64 * NW>(vt, vb, d.a.v_row, key0, p.nk, d.a.dim, d.vec);
-    __syncthreads();
-    if (key0 >= lim_hi && !dbias) continue;
+    for (int j = 0; j < J; ++j) g[j] = rows_times<T, DP>(vt, 32 * j, l31, h, gf, g[j]);
 #pragma unroll
-    for (int j = 0; j < BN / 32; ++j) {
-      f16v s, g;
+    for (int j = 0; j < J; ++j) {
+      finish_scores<T, BIAS>(d, s[j], key0 + 32 * j, h, rb.lim, part, bias);
+      if (part || BIAS) {                                    // what is masked may stand beside a do.v that is not finite
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = g[e] = 0.f;
-      s = rows_times<T, DP>(kt, 32 * j, l31, h, qf, s);
-      g = rows_times<T, DP>(vt, 32 * j, l31, h, gf, g);
-      finish_scores<T, BIAS>(d, s, key0 + 32 * j, h, lim, key0 + BN > lim_lo, bias);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float x = __builtin_amdgcn_exp2f((s[e] - base) * LOG2E) * inv;
-        s[e] = s[e] == NEG_INF ? 0.f : x * (g[e] - delta);
+        for (int e = 0; e < 16; ++e) g[j][e] = s[j][e] == NEG_INF ? 0.f : g[j][e];
       }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[j][e] = Probs<T, BIAS>::p(s[j][e], c, f.f0, f.f1);
+    }
+    if (one) {
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) delta = fmaf(s[j][e], g[j][e], delta);
+      delta = half_sum(delta);
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[j][e] *= g[j][e] - delta;
       if constexpr (BIAS) {
-        if (dbias && live) {
+        if (dbias && rb.live) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int key = key0 + 32 * j + 8 * (e >> 2) + 4 * h + (e & 3);
-            if (key < p.nk) dbias[key] = (T)s[e];
+            if (key < p.nk) dbias[key] = (T)s[j][e];
           }
         }
       }
-      cols_times<DP>(kt, 32 * j, lane, (const float*)&s, dq);
     }
+#pragma unroll
+    for (int j = 0; j < J; ++j) cols_times<DP>(kt, 32 * j, lane, (const float*)&s[j], dq);
+  };
+  for (int t = 0; t < ktiles; t += 2) {
+    __syncthreads();
+    if (t + 1 < ktiles) fetch(kt1, vt1, t + 1);
+    work(kt0, vt0, t);
+    if (t + 1 >= ktiles) break;
+    __syncthreads();
+    if (t + 2 < ktiles) fetch(kt0, vt0, t + 2);
+    work(kt1, vt1, t + 1);
   }
-  if (live) store_col<T, DP>((T*)d.a.dq + at * d.a.dim, h, d.a.dim, d.vec, dq, d.a.scale);
+  if (!rb.live) return;
+  store_col<T, DP>((T*)d.a.dq + at * d.a.dim, h, d.a.dim, d.vec, dq, d.a.scale);
+  if (h == 0) {
+    d.delta[st] = delta;
+    d.fac0[st] = f.f0;
+    if (!FAST<T, BIAS>) d.fac1[st] = f.f1;
+  }
 }
 
 // ---- backward: gradients of the keys and values ---------------------------------------------------------------------------------------------------
-// NW waves x 32 keys; the rows of all heads of the group in tiles of BR.  Rows down, keys across: the probability and ds tiles are second operands as
-// they stand, dv[d, key] += do[row, d] p[row, key], dk[d, key] += q[row, d] ds[row, key].
+// NW waves x 32 keys; the rows of all heads of the group in tiles of BR, the next one on its way.  Rows down, keys across: the probability and ds tiles
+// are second operands as they stand, dv[d, key] += do[row, d] p[row, key], dk[d, key] += q[row, d] ds[row, key].
+template <typename T, int DP, int NW, int BR, bool BIAS>
+struct RowTile {
+  __attribute__((aligned(16))) T q[BR * DP], g[BR * DP];
+  __attribute__((aligned(16))) float f0[BR], f1[FAST<T, BIAS> ? 4 : BR], delta[BR];
+  int64_t bias[BIAS ? BR : 1];
+};
+
 template <typename T, int DP, int NW, int BR, bool BIAS>
 __global__ __launch_bounds__(64 * NW) void dkv_kernel(Dev d) {
-  __shared__ __attribute__((aligned(16))) T qt[BR * DP], gt[BR * DP];
-  __shared__ __attribute__((aligned(16))) float sm[BR], sl[BR], sd[BR];
-  __shared__ __attribute__((aligned(16))) int slim[BR];
-  __shared__ int64_t sb[BIAS ? BR : 1];
-  const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5, wave = threadIdx.x / 64;
+  __shared__ RowTile<T, DP, NW, BR, BIAS> rt0, rt1;
+  constexpr int NT = 64 * NW, BM = 32 * NW, J = BR / 32;
+  const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
   int tile;
   const Place p = place(d, blockIdx.x, &tile);
-  constexpr int BM = 32 * NW;
   if (tile * BM >= p.nk) return;
-  const int key0 = tile * BM, key = key0 + wave * 32 + l31;
+  const int key0 = tile * BM, w0 = key0 + (threadIdx.x & ~63) / 2, key = w0 + l31;
   const bool live = key < p.nk;
-  const int64_t token = p.k0 + (live ? key : p.nk - 1), plane = (int64_t)d.a.heads * d.a.n_q;
+  const int64_t token = p.k0 + (live ? key : p.nk - 1);
+  // rows that see key j of the complex: from (j + n_queries - n_keys) group on (causal), all otherwise
+  auto rows_from = [&](int j) __attribute__((always_inline)) { return d.a.causal ? clampi(j + p.nq - p.nk, p.nq) * d.group : 0; };
+  const int rmin = rows_from(key), r_lo = __builtin_amdgcn_readfirstlane(rows_from(w0)), r_hi = __builtin_amdgcn_readfirstlane(rows_from(w0 + 31));
+  const int first = rows_from(key0) / BR, last = (p.rows + BR - 1) / BR;
+
+  auto fetch = [&](RowTile<T, DP, NW, BR, BIAS>& rt, int t) __attribute__((always_inline)) {
+    auto src = [&](int r) __attribute__((always_inline)) { return row_at(d, p, min(t * BR + r, p.rows - 1)); };
+    stage<T, DP, BR, NT>(rt.q, d.a.dim, d.vec, [&](int r) { const Row x = src(r); return (const T*)d.a.q + x.token * d.a.q_row + x.head * d.a.q_head; });
+    stage<T, DP, BR, NT>(rt.g, d.a.dim, d.vec, [&](int r) { const Row x = src(r); return (const T*)d.a.dout + x.token * d.a.dout_row + x.head * d.a.dout_head; });
+    if (threadIdx.x < BR) {
+      const Row x = src(threadIdx.x);
+      const int64_t st = (int64_t)x.head * d.a.n_q + x.token;
+      rt.f0[threadIdx.x] = d.fac0[st];
+      if constexpr (!FAST<T, BIAS>) rt.f1[threadIdx.x] = d.fac1[st];
+      rt.delta[threadIdx.x] = d.delta[st];
+      if constexpr (BIAS) rt.bias[threadIdx.x] = x.head * d.a.bias_head + (p.pair0 + (int64_t)x.i * p.nk) * d.a.bias_pair;
+    }
+  };
+  if (first < last) fetch(rt0, first);
+  zero_pad<T, DP, BR, NT>(rt0.q, d.a.dim);
+  zero_pad<T, DP, BR, NT>(rt0.g, d.a.dim);
+  zero_pad<T, DP, BR, NT>(rt1.q, d.a.dim);
+  zero_pad<T, DP, BR, NT>(rt1.g, d.a.dim);
+
   typename Tr<T>::frag kf[NC<T, DP> / 2], vf[NC<T, DP> / 2];
 #pragma unroll
   for (int s = 0; s < NC<T, DP> / 2; ++s) {
     kf[s] = load_chunk<T>((const T*)d.a.k + token * d.a.k_row + p.hk * d.a.k_head, 2 * s + h, d.a.dim, d.vec);
     vf[s] = load_chunk<T>((const T*)d.a.v + token * d.a.v_row + p.hk * d.a.v_head, 2 * s + h, d.a.dim, d.vec);
   }
+  const float c = FAST<T, BIAS> ? d.a.scale * LOG2E : LOG2E;
   f16v dk[DP / 32], dv[DP / 32];
+  zero<DP / 32>(dk);
+  zero<DP / 32>(dv);
+  auto work = [&](const RowTile<T, DP, NW, BR, BIAS>& rt, int t) __attribute__((always_inline)) {
+    const int r0 = t * BR;
+    if (r0 + BR <= r_lo || w0 >= p.nk) return;
+    const bool part = r0 < r_hi || r0 + BR > p.rows || w0 + 32 > p.nk;
 #pragma unroll
-  for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) dk[i][e] = dv[i][e] = 0.f;
-  // the first query that sees this block's first key
-  const int first = d.a.causal ? clampi(key0 + p.nq - p.nk, p.nq) * d.group / BR * BR : 0;
-  for (int r0 = first; r0 < p.rows; r0 += BR) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < BR * NC<T, DP>; i += 64 * NW) {
-      constexpr int N = NC<T, DP>;
-      const int rr = i / N, c = i % N;
-      const Row row = row_at(d, p, min(r0 + rr, p.rows - 1));
-      const int to = (rr * N + (c ^ sw<N>(rr))) * Tr<T>::CH;
-      *reinterpret_cast<typename Tr<T>::frag*>(qt + to) = load_chunk<T>((const T*)d.a.q + row.token * d.a.q_row + row.head * d.a.q_head, c, d.a.dim, d.vec);
-      *reinterpret_cast<typename Tr<T>::frag*>(gt + to) =
-          load_chunk<T>((const T*)d.a.dout + row.token * d.a.dout_row + row.head * d.a.dout_head, c, d.a.dim, d.vec);
-    }
-    for (int i = threadIdx.x; i < BR; i += 64 * NW) {
-      const Row row = row_at(d, p, min(r0 + i, p.rows - 1));
-      const int64_t st = (int64_t)row.head * d.a.n_q + row.token;
-      const float m = d.a.stats[st], l = d.a.stats[plane + st];
-      sm[i] = m == NEG_INF ? 0.f : m;
-      sl[i] = l == 0.f ? 0.f : 1.f / l;
-      sd[i] = d.delta[st];
-      slim[i] = r0 + i < p.rows ? keys_seen(d, p, row.i) : 0;
-      if constexpr (BIAS) sb[i] = row.head * d.a.bias_head + (p.pair0 + (int64_t)row.i * p.nk) * d.a.bias_pair;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < BR / 32; ++j) {
+    for (int j = 0; j < J; ++j) {
       f16v s, g;
+      zero<1>(&s);
+      zero<1>(&g);
+      s = rows_times<T, DP>(rt.q, 32 * j, l31, h, kf, s);
+      g = rows_times<T, DP>(rt.g, 32 * j, l31, h, vf, g);
+      if constexpr (!FAST<T, BIAS>) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = g[e] = 0.f;
-      s = rows_times<T, DP>(qt, 32 * j, l31, h, kf, s);
-      g = rows_times<T, DP>(gt, 32 * j, l31, h, vf, g);
+        for (int e = 0; e < 16; ++e) s[e] *= d.a.scale;
+      }
+      if (part || BIAS) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int rr = 32 * j + 8 * (e >> 2) + 4 * h + (e & 3), r = r0 + rr;
+          bool seen = live && r >= rmin && r < p.rows;
+          if constexpr (BIAS) {
+            const float bv = seen ? (float)((const T*)d.a.bias)[rt.bias[rr] + key * d.a.bias_pair] : NEG_INF;
+            s[e] += bv;
+            seen = bv != NEG_INF;
+          }
+          s[e] = seen ? s[e] : NEG_INF;
+          g[e] = seen ? g[e] : 0.f;
+        }
+      }
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int rr = 32 * j + 8 * (e >> 2) + 4 * h + (e & 3);
-        const bool seen = live && key < slim[rr];
-        float x = s[e] * d.a.scale;
-        if constexpr (BIAS) {
-          const float bv = seen ? (float)((const T*)d.a.bias)[sb[rr] + key * d.a.bias_pair] : NEG_INF;
-          x = bv == NEG_INF ? NEG_INF : x + bv;
-        } else {
-          x = seen ? x : NEG_INF;
-        }
-        const float pr = __builtin_amdgcn_exp2f((x - sm[rr]) * LOG2E) * sl[rr];
-        s[e] = x == NEG_INF ? 0.f : pr;
-        g[e] = x == NEG_INF ? 0.f : pr * (g[e] - sd[rr]);
+        s[e] = Probs<T, BIAS>::p(s[e], c, rt.f0[rr], FAST<T, BIAS> ? 0.f : rt.f1[rr]);
+        g[e] = s[e] * (g[e] - rt.delta[rr]);
       }
-      cols_times<DP>(gt, 32 * j, lane, (const float*)&s, dv);
-      cols_times<DP>(qt, 32 * j, lane, (const float*)&g, dk);
+      cols_times<DP>(rt.g, 32 * j, lane, (const float*)&s, dv);
+      cols_times<DP>(rt.q, 32 * j, lane, (const float*)&g, dk);
     }
+  };
+  for (int t = first; t < last; t += 2) {
+    __syncthreads();
+    if (t + 1 < last) fetch(rt1, t + 1);
+    work(rt0, t);
+    if (t + 1 >= last) break;
+    __syncthreads();
+    if (t + 2 < last) fetch(rt0, t + 2);
+    work(rt1, t + 1);
   }
   if (live) {
     const int64_t at = (token * d.a.kv_heads + p.hk) * d.a.dim;
@@ -362,7 +496,7 @@ hipError_t run_fwd(const Dev& d, bool small, hipStream_t st) {
 
 template <typename T, int DP>
 hipError_t run_bwd(const Dev& d0, bool small_rows, bool small_keys, hipStream_t st) {
-  constexpr int BN = sizeof(T) == 2 ? 64 : 32, BR = 32;
+  constexpr int BN = sizeof(T) == 2 ? 64 : 32, BR = BN;
   Dev d = d0;
   const int64_t rows = (int64_t)d.a.max_nq * d.group;
   d.tiles = (int)((rows + (small_rows ? 31 : 127)) / (small_rows ? 32 : 128));
