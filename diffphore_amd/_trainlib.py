@@ -54,7 +54,7 @@ def lib():
         L.dpt_layer_norm_bwd.argtypes = [i32, i32, i64, i32, P, i64, P, i64, P, P, P, P, i64, P, P, P, C.c_size_t, P]
         L.dpt_attn_ws_bytes.argtypes, L.dpt_attn_ws_bytes.restype = [C.POINTER(DptAttnArgs), i32], C.c_size_t
         L.dpt_attn_fwd.argtypes = L.dpt_attn_bwd.argtypes = [C.POINTER(DptAttnArgs), P]
-        L.dpt_adamw_step.argtypes = [C.POINTER(DptAdamWArgs), C.POINTER(P), P]
+        L.dpt_adamw_step.argtypes = [C.POINTER(DptAdamWArgs), P, P]           # grads: address of a host array of device addresses
         L.dpt_adamw_moments.argtypes = [P, P, P, P, i32, P, P, P]
         _lib = L
     return _lib
@@ -68,21 +68,19 @@ def check(rc: int, what: str):
         raise DiffPhoreLibraryError(f"{what} failed with code {rc}" + (f" ({_WHY[rc]})" if rc in _WHY else ""))
 
 
-class on:
-    """The stream that work on `device` is enqueued on (its current stream), with that device current for the launch."""
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
-    def __init__(self, device: torch.device):
-        self.index = device.index
-        self.guard = torch.cuda.device(device) if torch.cuda.current_device() != device.index else None
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream(self.index).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def call(what: str, fn, index: int, *args):
+    """fn(*args, stream) on the current stream of GPU `index`, with that device current for the launch; a code other than 0 is an error.  (Called for every
+    operator: the common case - the tensors' device is the current one - costs half a microsecond beside the launch.)"""
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc, what)
 
 
 def need_gpu(t: torch.Tensor, name: str):

@@ -98,7 +98,7 @@ __device__ __forceinline__ void zero(f16v* x) {
 // running base and sum per row.  The base follows the row's maximum only when that has moved by more than 2^8 (exp of the difference then still has all its
 // bits, and so has a bf16 of it), so the accumulators are rescaled a few times per row instead of once per tile.
 template <typename T, int DP, int NW, int BN, bool BIAS>
-__global__ __launch_bounds__(64 * NW) void fwd_kernel(Dev d) {
+__global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void fwd_kernel(Dev d) {
   __shared__ __attribute__((aligned(16))) T kt0[BN * DP], vt0[BN * DP], kt1[BN * DP], vt1[BN * DP];
   constexpr int NT = 64 * NW, BM = 32 * NW, J = BN / 32;
   constexpr float FAR = 8.f;
@@ -247,7 +247,7 @@ struct Probs {
 // rows' factors for the second kernel.  Where a complex's keys are one tile, delta is taken as sum_j p_j do.v_j instead: the stored out is rounded to
 // its type, and with few keys that rounding does not average out.
 template <typename T, int DP, int NW, int BN, bool BIAS>
-__global__ __launch_bounds__(64 * NW) void dq_kernel(Dev d) {
+__global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dq_kernel(Dev d) {
   __shared__ __attribute__((aligned(16))) T kt0[BN * DP], vt0[BN * DP], kt1[BN * DP], vt1[BN * DP];
   constexpr int NT = 64 * NW, BM = 32 * NW, J = BN / 32;
   const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
@@ -307,46 +307,46 @@ __global__ __launch_bounds__(64 * NW) void dq_kernel(Dev d) {
     const int key0 = t * BN;
     if (key0 >= rb.lim_hi && !dbias) return;
     const bool part = key0 + BN > rb.lim_lo;
-    f16v s[J], g[J];
-    zero<J>(s);
-    zero<J>(g);
-#pragma unroll
-    for (int j = 0; j < J; ++j) s[j] = rows_times<T, DP>(kt, 32 * j, l31, h, qf, s[j]);
-#pragma unroll
-    for (int j = 0; j < J; ++j) g[j] = rows_times<T, DP>(vt, 32 * j, l31, h, gf, g[j]);
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      finish_scores<T, BIAS>(d, s[j], key0 + 32 * j, h, rb.lim, part, bias);
+    // probabilities (into s) and do.v (into g) of 32 keys
+    auto probs = [&](int j, f16v& s, f16v& g) __attribute__((always_inline)) {
+      zero<1>(&s);
+      zero<1>(&g);
+      s = rows_times<T, DP>(kt, 32 * j, l31, h, qf, s);
+      g = rows_times<T, DP>(vt, 32 * j, l31, h, gf, g);
+      finish_scores<T, BIAS>(d, s, key0 + 32 * j, h, rb.lim, part, bias);
       if (part || BIAS) {                                    // what is masked may stand beside a do.v that is not finite
 #pragma unroll
-        for (int e = 0; e < 16; ++e) g[j][e] = s[j][e] == NEG_INF ? 0.f : g[j][e];
+        for (int e = 0; e < 16; ++e) g[e] = s[e] == NEG_INF ? 0.f : g[e];
       }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[j][e] = Probs<T, BIAS>::p(s[j][e], c, f.f0, f.f1);
-    }
+      for (int e = 0; e < 16; ++e) s[e] = Probs<T, BIAS>::p(s[e], c, f.f0, f.f1);
+    };
+    f16v s, g;
     if (one) {
+#pragma unroll 1
+      for (int j = 0; j < J; ++j) {
+        probs(j, s, g);
 #pragma unroll
-      for (int j = 0; j < J; ++j)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) delta = fmaf(s[j][e], g[j][e], delta);
+        for (int e = 0; e < 16; ++e) delta = fmaf(s[e], g[e], delta);
+      }
       delta = half_sum(delta);
     }
 #pragma unroll
     for (int j = 0; j < J; ++j) {
+      probs(j, s, g);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[j][e] *= g[j][e] - delta;
+      for (int e = 0; e < 16; ++e) s[e] *= g[e] - delta;
       if constexpr (BIAS) {
         if (dbias && rb.live) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int key = key0 + 32 * j + 8 * (e >> 2) + 4 * h + (e & 3);
-            if (key < p.nk) dbias[key] = (T)s[j][e];
+            if (key < p.nk) dbias[key] = (T)s[e];
           }
         }
       }
+      cols_times<DP>(kt, 32 * j, lane, (const float*)&s, dq);
     }
-#pragma unroll
-    for (int j = 0; j < J; ++j) cols_times<DP>(kt, 32 * j, lane, (const float*)&s[j], dq);
   };
   for (int t = 0; t < ktiles; t += 2) {
     __syncthreads();
@@ -377,7 +377,7 @@ struct RowTile {
 };
 
 template <typename T, int DP, int NW, int BR, bool BIAS>
-__global__ __launch_bounds__(64 * NW) void dkv_kernel(Dev d) {
+__global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dkv_kernel(Dev d) {
   __shared__ RowTile<T, DP, NW, BR, BIAS> rt0, rt1;
   constexpr int NT = 64 * NW, BM = 32 * NW, J = BR / 32;
   const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;

@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _trainlib
-from ._trainlib import TYPES, DptAttnArgs, check, need_gpu, on
+from ._trainlib import TYPES, DptAttnArgs, call, need_gpu
 
 _LN_MAX_WIDTH = 16384
 
@@ -30,12 +30,16 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return y if y.stride(1) == 1 or y.shape[1] == 1 else y.contiguous()
 
 
+def _empty_like(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def _row_stride(x2: torch.Tensor) -> int:
     return x2.stride(0) if x2.shape[0] > 1 else x2.shape[1]
 
 
 def _check_affine(x, p, name):
-    if p is None:
+    if p is None or (type(p) is torch.Tensor and p.dtype is x.dtype and p.shape == x.shape[-1:] and p.device == x.device and p.is_contiguous()):
         return
     need_gpu(p, name)
     if p.device != x.device:
@@ -69,13 +73,13 @@ def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, b
     L = _trainlib.lib()
     x2 = _rows(x)
     rows, width = x2.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+    y = _empty_like(x)
+    mean = torch.empty(rows, dtype=torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
     w = weight if weight is not None else bias
-    with on(x.device) as stream:
-        check(L.dpt_layer_norm_fwd(TYPES[x.dtype], TYPES[w.dtype if w is not None else x.dtype], rows, width, x2.data_ptr(), _row_stride(x2),
-                                   weight.data_ptr() if weight is not None else None, bias.data_ptr() if bias is not None else None, eps,
-                                   y.data_ptr(), width, mean.data_ptr(), rstd.data_ptr(), stream), "dpt_layer_norm_fwd")
+    call("dpt_layer_norm_fwd", L.dpt_layer_norm_fwd, x.get_device(), TYPES[x.dtype], TYPES[w.dtype if w is not None else x.dtype], rows, width, x2.data_ptr(),
+         _row_stride(x2), weight.data_ptr() if weight is not None else None, bias.data_ptr() if bias is not None else None, eps, y.data_ptr(), width,
+         mean.data_ptr(), rstd.data_ptr())
     return y, mean, rstd
 
 
@@ -96,16 +100,17 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     wtype = weight.dtype if weight is not None else param_dtype or x.dtype
     if wtype != x.dtype and wtype != torch.float32:
         raise TypeError(f"param_dtype {wtype}: x's type ({x.dtype}) or float32")
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = _empty_like(x)
     dw = db = ws = None
+    n = 0
     if want_params:
-        dw, db = torch.empty((2, width), dtype=wtype, device=x.device)
-        ws = torch.empty(L.dpt_layer_norm_ws_bytes(rows, width), dtype=torch.uint8, device=x.device)
-    with on(x.device) as stream:
-        check(L.dpt_layer_norm_bwd(TYPES[x.dtype], TYPES[wtype], rows, width, dy2.data_ptr(), _row_stride(dy2), x2.data_ptr(), _row_stride(x2),
-                                   mean.data_ptr(), rstd.data_ptr(), weight.data_ptr() if weight is not None else None, dx.data_ptr(), width,
-                                   dw.data_ptr() if want_params else None, db.data_ptr() if want_params else None,
-                                   ws.data_ptr() if want_params else None, ws.numel() if want_params else 0, stream), "dpt_layer_norm_bwd")
+        dw = torch.empty_like(weight) if weight is not None else torch.empty(width, dtype=wtype, device=x.device)
+        db = torch.empty_like(dw)
+        n = L.dpt_layer_norm_ws_bytes(rows, width)
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+    call("dpt_layer_norm_bwd", L.dpt_layer_norm_bwd, x.get_device(), TYPES[x.dtype], TYPES[wtype], rows, width, dy2.data_ptr(), _row_stride(dy2), x2.data_ptr(),
+         _row_stride(x2), mean.data_ptr(), rstd.data_ptr(), weight.data_ptr() if weight is not None else None, dx.data_ptr(), width,
+         dw.data_ptr() if want_params else None, db.data_ptr() if want_params else None, ws.data_ptr() if want_params else None, n)
     return dx, dw, db
 
 
@@ -185,9 +190,9 @@ def _check_attn(q, k, v, plan, bias, scale):
         need_gpu(t, name)
         if t.dim() != 3:
             raise ValueError(f"{name} has shape {tuple(t.shape)}: [rows, heads, dim] is wanted")
-        if t.dtype != q.dtype or t.device != q.device:
+        if t.dtype is not q.dtype or t.get_device() != q.get_device():
             raise ValueError(f"{name} is {t.dtype} on {t.device}, q is {q.dtype} on {q.device}")
-    if plan.device != q.device:
+    if plan.device.index != q.get_device():
         raise ValueError(f"the plan is on {plan.device}, q on {q.device}")
     heads, dim = q.shape[1:]
     if k.shape != v.shape or k.shape[2] != dim:
@@ -237,7 +242,7 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: P
     _check_attn(q, k, v, plan, bias, scale)
     L = _trainlib.lib()
     q, k, v = _unit(q), _unit(k), _unit(v)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = _empty_like(q)
     stats = torch.empty((2, q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
     a = _attn_args(q, k, v, plan, bias, causal, scale)
     a.out, a.stats = out.data_ptr(), stats.data_ptr()
@@ -245,8 +250,7 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: P
     if n:
         ws = torch.empty(n, dtype=torch.uint8, device=q.device)
         a.ws, a.ws_bytes = ws.data_ptr(), n
-    with on(q.device) as stream:
-        check(L.dpt_attn_fwd(C.byref(a), stream), "dpt_attn_fwd")
+    call("dpt_attn_fwd", L.dpt_attn_fwd, q.get_device(), C.byref(a))
     return out, stats
 
 
@@ -264,8 +268,8 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
         raise ValueError(f"stats is {tuple(stats.shape)} {stats.dtype} on {stats.device}: attention_forward's is wanted")
     L = _trainlib.lib()
     q, k, v, dout, out, stats = _unit(q), _unit(k), _unit(v), _unit(dout), out.contiguous(), stats.contiguous()
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    dbias = torch.empty(bias.shape, dtype=bias.dtype, device=bias.device) if bias is not None and want_bias else None
+    dq, dk, dv = _empty_like(q), _empty_like(k), _empty_like(v)
+    dbias = _empty_like(bias) if bias is not None and want_bias else None
     a = _attn_args(q, k, v, plan, bias, causal, scale)
     a.dout_row, a.dout_head, _ = dout.stride()
     a.out, a.stats, a.dout, a.dq, a.dk, a.dv = (t.data_ptr() for t in (out, stats, dout, dq, dk, dv))
@@ -275,8 +279,7 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     if n:
         ws = torch.empty(n, dtype=torch.uint8, device=q.device)
         a.ws, a.ws_bytes = ws.data_ptr(), n
-    with on(q.device) as stream:
-        check(L.dpt_attn_bwd(C.byref(a), stream), "dpt_attn_bwd")
+    call("dpt_attn_bwd", L.dpt_attn_bwd, q.get_device(), C.byref(a))
     return dq, dk, dv, dbias
 
 

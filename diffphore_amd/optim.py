@@ -7,16 +7,19 @@ model takes for a validation run (`fit.inference_epoch`).  All arithmetic runs i
 from __future__ import annotations
 
 import ctypes as C
+from array import array
+from operator import attrgetter
 from typing import Iterable, Optional
 
 import numpy as np
 import torch
 
 from . import _trainlib
-from ._trainlib import TYPES, DptAdamWArgs, check, need_gpu, on
+from ._trainlib import TYPES, DptAdamWArgs, call, need_gpu
 
 BLOCK = 256                # elements of a tensor that share one scale of an 8-bit state; every tensor's slot in the flat buffers is a multiple of it
 _MAX_TENSORS = 400         # per launch
+_DTYPE = attrgetter("dtype")
 
 
 class AdamW:
@@ -68,7 +71,7 @@ class AdamW:
             if (n not in index) if index is not None else not 0 <= int(n) < len(params):
                 raise ValueError(f"no_decay: there is no parameter {n!r}")
             decay[index[n] if index is not None else int(n)] = 0.0
-        self._numel = [p.numel() for p in params]
+        self._numel, self._sizes = [p.numel() for p in params], [p.shape for p in params]
         blocks = [-(-n // BLOCK) for n in self._numel]
         self.first_block = [0]
         for b in blocks:
@@ -115,9 +118,8 @@ class AdamW:
         if self.state_bits == 32:
             return self.exp_avg, self.exp_avg_sq
         m, v = torch.empty((2, self.n_blocks * BLOCK), dtype=torch.float32, device=self.device)
-        with on(self.device) as stream:
-            check(_trainlib.lib().dpt_adamw_moments(self.exp_avg.data_ptr(), self.exp_avg_scale.data_ptr(), self.exp_avg_sq.data_ptr(),
-                                                    self.exp_avg_sq_scale.data_ptr(), self.n_blocks, m.data_ptr(), v.data_ptr(), stream), "dpt_adamw_moments")
+        call("dpt_adamw_moments", _trainlib.lib().dpt_adamw_moments, self.device.index, self.exp_avg.data_ptr(), self.exp_avg_scale.data_ptr(),
+             self.exp_avg_sq.data_ptr(), self.exp_avg_sq_scale.data_ptr(), self.n_blocks, m.data_ptr(), v.data_ptr())
         return m, v
 
     # ---- checkpoints ----------------------------------------------------------------------------------------------------
@@ -166,35 +168,35 @@ class AdamW:
         tensor on the device.  grad_scale: a float32 tensor on the device that multiplies the gradients."""
         if grads is None:
             grads = [p.grad for p in self.params]
-        elif isinstance(grads, dict):
+        elif not isinstance(grads, (list, dict)):
+            grads = list(grads)
+        if isinstance(grads, dict):
             if self.names is None or grads.keys() - set(self.names):
                 raise ValueError("grads names tensors that are not parameters")
             grads = [grads.get(n) for n in self.names]
         if len(grads) != len(self.params):
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
-        gtype, index, ptrs = None, self.device.index, []
-        for i, (g, p) in enumerate(zip(grads, self._alias)):
-            if g is None:
-                ptrs.append(0)
-                continue
-            if g.dtype is not gtype:
-                if gtype is not None or g.dtype not in (self.dtype, torch.float32):
-                    raise TypeError(f"gradient {i} is {g.dtype}: all in {self.dtype}, or all in float32")
-                gtype = g.dtype
-            if g.shape != p.shape or g.get_device() != index or not g.is_contiguous():
-                raise ValueError(f"gradient {i} is {tuple(g.shape)} on {g.device}: contiguous {tuple(p.shape)} on {self.device} is wanted")
-            ptrs.append(g.data_ptr())
+        # one pass per property over the whole list: some hundreds of small tensors are the common case, and a loop over all of them costs more than the step
+        some = grads if type(None) not in set(map(type, grads)) else [g for g in grads if g is not None]
+        types = set(map(_DTYPE, some)) or {self.dtype}
+        if len(types) > 1 or not types <= {self.dtype, torch.float32}:
+            raise TypeError(f"gradients in {types}: all in {self.dtype}, or all in float32")
+        sizes = self._sizes if some is grads else [s for s, g in zip(self._sizes, grads) if g is not None]
+        if [g.shape for g in some] != sizes or not set(map(torch.Tensor.get_device, some)) <= {self.device.index} or not all(map(torch.Tensor.is_contiguous, some)):
+            for i, (g, s) in enumerate(zip(grads, self._sizes)):
+                if g is not None and (g.shape != s or g.get_device() != self.device.index or not g.is_contiguous()):
+                    raise ValueError(f"gradient {i} is {tuple(g.shape)} on {g.device}: contiguous {tuple(s)} on {self.device} is wanted")
+        ptrs = list(map(torch.Tensor.data_ptr, grads)) if some is grads else [g.data_ptr() if g is not None else 0 for g in grads]
         L = _trainlib.lib()
         a = self._args
-        a.grad_type = TYPES[gtype or self.dtype]
+        a.grad_type = TYPES[types.pop()]
         a.lr_dev, a.lr = (self._scalar(lr, "lr"), 0.0) if isinstance(lr, torch.Tensor) else (None, self.lr if lr is None else float(lr))
         a.grad_scale = self._scalar(grad_scale, "grad_scale") if grad_scale is not None else None
-        with on(self.device) as stream:
-            for i in range(0, len(ptrs), _MAX_TENSORS):
-                part = ptrs[i:i + _MAX_TENSORS]
-                a.tensor0, a.n_tensors, a.block0, a.last = i, len(part), self.first_block[i], int(i + len(part) == len(ptrs))
-                a.n_blocks = self.first_block[i + len(part)] - a.block0
-                check(L.dpt_adamw_step(C.byref(a), (C.c_void_p * len(part))(*part), stream), "dpt_adamw_step")
+        for i in range(0, len(ptrs), _MAX_TENSORS):
+            part = array("Q", ptrs[i:i + _MAX_TENSORS])
+            a.tensor0, a.n_tensors, a.block0, a.last = i, len(part), self.first_block[i], int(i + len(part) == len(ptrs))
+            a.n_blocks = self.first_block[i + len(part)] - a.block0
+            call("dpt_adamw_step", L.dpt_adamw_step, self.device.index, C.byref(a), part.buffer_info()[0])
 
     def zero_grad(self):
         for p in self.params:
