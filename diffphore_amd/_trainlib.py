@@ -28,9 +28,8 @@ class DptAttnArgs(C.Structure):
 class DptAdamWArgs(C.Structure):
     _fields_ = ([(n, i32) for n in ("type", "grad_type", "state_bits", "n_tensors", "block0", "n_blocks", "last")]
                 + [(n, f64) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "ema_decay")]
-                + [(n, P) for n in ("lr_dev", "grad_scale", "block_tensor")] + [("tensor0", i32), ("pad_", i32)]
-                + [(n, P) for n in ("first_block", "numel", "param", "decay", "master", "ema", "exp_avg", "exp_avg_sq", "exp_avg_scale",
-                                    "exp_avg_sq_scale", "counter")])
+                + [(n, P) for n in ("lr_dev", "grad_scale", "blocks")] + [("tensor0", i32), ("pad_", i32)]
+                + [(n, P) for n in ("master", "ema", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "counter")])
 
 
 _lib = None

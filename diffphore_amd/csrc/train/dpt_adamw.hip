@@ -7,9 +7,12 @@
 // have read them moves them on.
 //
 // 8-bit states: m' and v' are formed in 64 bits from the decoded values, the parameter's update uses them unrounded, and the stored codes are the
-// nearest ones.  "Nearest" is decided exactly: a candidate from a 32-bit root is compared with the borders (c -+ 1/2)^2 resp. ^4, whose products
-// with the scale are exact or within 2^-53 - so a code never depends on the rounding of a square root.
+// nearest ones.  "Nearest" is decided exactly: a 32-bit root gives the code's position, and where some position of the block lies within its own error of a
+// border between two codes, the block's values are compared with the borders in 64 bits, (c - 1/2)^2 resp. ^4 times the scale (exact, or within 2^-53) -
+// so a code does not depend on the rounding of a root.  This form is bound by instructions as much as by memory: everything that can be is 32 bits.
 #include "dpt_dev.h"
+
+#include <type_traits>
 
 namespace dpta {
 using namespace dpt;
@@ -18,139 +21,213 @@ constexpr int BLOCK = DPT_ADAMW_BLOCK, WAVES = 4;
 
 struct Grads { const void* p[DPT_ADAMW_MAX_TENSORS]; };
 
-__device__ __forceinline__ double wave_max(double x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double y = __shfl_xor(x, d, 64);
-    x = y > x ? y : x;
-  }
-  return x;
+// maximum over the wave of values >= 0, without LDS: shifts inside rows of 16 lanes, then across rows; lane 63 has it in the end
+__device__ __forceinline__ float wave_max(float x) {
+  auto step = [&](auto ctrl) __attribute__((always_inline)) {
+    const int b = __builtin_bit_cast(int, x);
+    x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(b, b, decltype(ctrl)::value, 0xf, 0xf, false)));
+  };
+  step(std::integral_constant<int, 0x111>{});   // row_shr 1, 2, 4, 8
+  step(std::integral_constant<int, 0x112>{});
+  step(std::integral_constant<int, 0x114>{});
+  step(std::integral_constant<int, 0x118>{});
+  step(std::integral_constant<int, 0x142>{});   // row_bcast 15, 31
+  step(std::integral_constant<int, 0x143>{});
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
 
-// nearest code c in 0..TOP of |x| on the curve scale (c / TOP)^POW
+// Position t = TOP (x / scale)^(1/POW) of a value on its curve.  x (rounded from 64 bits) and its product with 1 / scale are good to 2^-24, 1 / scale and a root
+// to an ulp, so |dt| < TOP 2^-24 (4 / POW + 3) < 8e-5 on both curves (NEAR); below TINY the 32-bit values may have lost bits to underflow.
+constexpr float NEAR = 1e-4f, TINY = 1e-30f;
 template <int TOP, int POW>
-__device__ __forceinline__ int encode(double x, float scale, double inv) {
-  constexpr double T = POW == 2 ? (double)TOP * TOP : (double)TOP * TOP * TOP * TOP;
-  const float u = (float)(x * inv);
-  float root = sqrtf(u);
-  if constexpr (POW == 4) root = sqrtf(root);
-  int c = (int)(root * (float)TOP + 0.5f);
-  c = c > TOP ? TOP : c;
-  const double y = x * T, s = scale;
-  auto border = [&](int k) {                       // scale (k - 1/2)^POW
-    const double h = (double)k - 0.5, h2 = h * h;
-    return POW == 2 ? s * h2 : s * (h2 * h2);
-  };
-  if (c < TOP && y >= border(c + 1)) ++c;
-  else if (c > 0 && y < border(c)) --c;
-  return c;
+__device__ __forceinline__ float position(float x, float inv) {
+  float t = __builtin_amdgcn_sqrtf(x * inv);
+  if constexpr (POW == 4) t = __builtin_amdgcn_sqrtf(t);
+  return t * (float)TOP;
 }
+__device__ __forceinline__ bool near_border(float t) { return fabsf(__builtin_amdgcn_fractf(t + 0.5f) - 0.5f) > 0.5f - NEAR; }
+
+// Nearest code by comparison with the borders; for values whose root may be off, from a 64-bit root
+template <int TOP, int POW>
+__device__ __forceinline__ int exact_code(double x, double scale) {
+  constexpr double T = POW == 2 ? (double)TOP * TOP : (double)TOP * TOP * TOP * TOP;
+  double t = sqrt(x / scale);
+  if constexpr (POW == 4) t = sqrt(t);
+  const int near = (int)(t * TOP + 0.5);           // right, or one too high or too low by a rounding
+  const int c = near > TOP ? TOP : near;
+  auto below = [&](int k) { const double h = (double)k - 0.5, h2 = h * h; return x * T < scale * (POW == 2 ? h2 : h2 * h2); };
+  return c > 0 && below(c) ? c - 1 : c < TOP && !below(c + 1) ? c + 1 : c;
+}
+
+// a block's values on their way
+template <typename P, typename G>
+struct Values {
+  typedef __attribute__((ext_vector_type(4))) G g4;
+  DptAdamWBlock b;
+  const G* g;                    // nullptr: no gradient, the tensor and its state stay as they are
+  bool whole;                    // 256 elements at aligned addresses
+  g4 gv;
+  f4 pv, mv, vv, ev;
+  int mc, vc;                    // four codes each
+  float ms, vs;
+};
 
 template <typename P, typename G, int BITS, bool EMA>
-__global__ __launch_bounds__(64 * WAVES) void step_kernel(DptAdamWArgs a, Grads grads) {
+__global__ __launch_bounds__(64 * WAVES, 6) void step_kernel(DptAdamWArgs a, Grads grads) {
   // the step's factors, in 64 bits
   const double p1 = a.counter[1] * a.beta1, p2 = a.counter[2] * a.beta2;
   const double lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
   const float b1 = (float)a.beta1, omb1 = (float)(1.0 - a.beta1), b2 = (float)a.beta2, omb2 = (float)(1.0 - a.beta2);
   const float lr1 = (float)(lr / (1.0 - p1)), ic2 = (float)(1.0 / (1.0 - p2)), eps = (float)a.eps;
   const float ema_d = (float)a.ema_decay, ema_o = (float)(1.0 - a.ema_decay), gs = a.grad_scale ? *a.grad_scale : 1.f;
+  const double k1 = (double)gs * (1.0 - a.beta1), k2 = (double)gs * (double)gs * (1.0 - a.beta2);
   const int lane = threadIdx.x & 63;
-  for (int i = blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / 64); i < a.n_blocks; i += gridDim.x * WAVES) {
-    const int blk = a.block0 + i, t = __builtin_amdgcn_readfirstlane(a.block_tensor[blk]);
-    const int64_t in_tensor = (int64_t)(blk - a.first_block[t]) * BLOCK, at = (int64_t)blk * BLOCK + lane * 4;
-    const int64_t left = a.numel[t] - in_tensor;                         // elements of the tensor from this block on
-    P* __restrict__ p = (P*)a.param[t] + in_tensor;
-    const G* __restrict__ g = (const G*)grads.p[t - a.tensor0] + in_tensor;
-    const float shrink = (float)(1.0 - lr * a.weight_decay * (double)a.decay[t]);
-    const bool whole = left >= BLOCK && ((uintptr_t)p % (4 * sizeof(P))) == 0 && ((uintptr_t)g % (4 * sizeof(G))) == 0;
-    if (!grads.p[t - a.tensor0]) continue;                               // no gradient: the tensor and its state stay as they are
-    float gv[4], pv[4];
-    if (whole) {
-      load_n<G, 4>(g + lane * 4, gv);
-      if constexpr (sizeof(P) == 4) load_n<P, 4>(p + lane * 4, pv);
+  typedef const __attribute__((address_space(4))) DptAdamWBlock* Rec;      // constant memory: a wave's record is one scalar load
+  auto record = [&](int i) __attribute__((always_inline)) {
+    const Rec r = (Rec)(unsigned long long)(a.blocks + a.block0 + min(i, a.n_blocks - 1));
+    return DptAdamWBlock{r->param, r->tensor, r->index, r->left, r->decay, {0, 0}};
+  };
+  auto fetch = [&](int i, const DptAdamWBlock& b) __attribute__((always_inline)) {
+    Values<P, G> x;
+    x.b = b;
+    const G* g = (const G*)grads.p[b.tensor - a.tensor0];
+    x.g = g && i < a.n_blocks ? g + (int64_t)b.index * BLOCK : nullptr;
+    x.whole = b.left == BLOCK && b.param % (4 * sizeof(P)) == 0 && (uintptr_t)g % (4 * sizeof(G)) == 0;
+    if (!x.g) return x;
+    const P* p = (const P*)b.param;
+    const int64_t blk = a.block0 + i, at = blk * BLOCK + lane * 4;
+    if (x.whole) {
+      x.gv = *(const typename Values<P, G>::g4*)(x.g + lane * 4);
+      if constexpr (sizeof(P) == 4) x.pv = *(const f4*)(p + lane * 4);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const bool in = lane * 4 + e < left;
-        gv[e] = in ? (float)g[lane * 4 + e] : 0.f;
-        if constexpr (sizeof(P) == 4) pv[e] = in ? (float)p[lane * 4 + e] : 0.f;
+        const bool in = lane * 4 + e < b.left;
+        x.gv[e] = in ? x.g[lane * 4 + e] : (G)0.f;
+        if constexpr (sizeof(P) == 4) x.pv[e] = in ? p[lane * 4 + e] : 0.f;
       }
     }
-    if constexpr (sizeof(P) == 2) load_n<float, 4>(a.master + at, pv);
-    float mv[4], vv[4];
+    if constexpr (sizeof(P) == 2) x.pv = *(const f4*)(a.master + at);
+    if constexpr (EMA) x.ev = *(const f4*)(a.ema + at);
     if constexpr (BITS == 32) {
-      float* ms = (float*)a.exp_avg + at;
-      float* vs = (float*)a.exp_avg_sq + at;
-      load_n<float, 4>(ms, mv);
-      load_n<float, 4>(vs, vv);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = gv[e] * gs;
-        mv[e] = mv[e] * b1 + x * omb1;
-        vv[e] = vv[e] * b2 + x * x * omb2;
-      }
-      store_n<float, 4>(ms, mv);
-      store_n<float, 4>(vs, vv);
+      x.mv = *(const f4*)((const float*)a.exp_avg + at);
+      x.vv = *(const f4*)((const float*)a.exp_avg_sq + at);
     } else {
-      char4* ms = (char4*)((int8_t*)a.exp_avg + at);
-      uchar4* vs = (uchar4*)((uint8_t*)a.exp_avg_sq + at);
-      const char4 mc = *ms;
-      const uchar4 vc = *vs;
-      const double ma = (double)a.exp_avg_scale[blk] / (127.0 * 127.0), va = (double)a.exp_avg_sq_scale[blk] / (255.0 * 255.0 * 255.0 * 255.0);
-      const int ci[4] = {mc.x, mc.y, mc.z, mc.w}, ui[4] = {vc.x, vc.y, vc.z, vc.w};
-      double m[4], v[4], mm = 0.0, vm = 0.0;
-      bool fine = true;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const double x = (double)gv[e] * (double)gs;
-        const int u2 = ui[e] * ui[e];                                     // < 2^16: its square fits 32 unsigned bits
-        m[e] = ma * (double)(ci[e] * abs(ci[e])) * a.beta1 + x * (1.0 - a.beta1);
-        v[e] = va * (double)((unsigned)u2 * (unsigned)u2) * a.beta2 + x * x * (1.0 - a.beta2);
-        mv[e] = (float)m[e];
-        vv[e] = (float)v[e];
-        fine = fine && __builtin_isfinite(mv[e]) && __builtin_isfinite(vv[e]);
-        mm = fmax(mm, fabs(m[e]));
-        vm = fmax(vm, v[e]);
-      }
-      float msc = (float)wave_max(mm), vsc = (float)wave_max(vm);
-      int cm[4] = {0, 0, 0, 0}, cv[4] = {0, 0, 0, 0};
-      if (__all(fine)) {
-        const double mi = 1.0 / (double)msc, vi = 1.0 / (double)vsc;         // inf for a scale of 0: not used then
+      x.mc = *(const int*)((const int8_t*)a.exp_avg + at);
+      x.vc = *(const int*)((const uint8_t*)a.exp_avg_sq + at);
+      x.ms = a.exp_avg_scale[blk];
+      x.vs = a.exp_avg_sq_scale[blk];
+    }
+    return x;
+  };
+  // the next block's values are on their way while a block is worked on, and the record of the one after it: otherwise every turn would wait for a
+  // record and then for the values that it points to
+  const int stride = gridDim.x * WAVES;
+  int i = blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  Values<P, G> x = fetch(i, record(i));
+  DptAdamWBlock ahead = record(i + stride);
+  for (; i < a.n_blocks; i += stride) {
+    const Values<P, G> next = fetch(i + stride, ahead);
+    ahead = record(i + 2 * stride);
+    if (x.g) {
+      const int64_t blk = a.block0 + i, at = blk * BLOCK + lane * 4;
+      const float shrink = (float)(1.0 - lr * a.weight_decay * (double)x.b.decay);
+      P* p = (P*)x.b.param;
+      if constexpr (BITS == 32) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if (msc > 0.f) {
-            cm[e] = encode<127, 2>(fabs(m[e]), msc, mi);
-            if (m[e] < 0.0) cm[e] = -cm[e];
-          }
-          if (vsc > 0.f) {
-            cv[e] = encode<255, 4>(v[e], vsc, vi);
-            if (cv[e] == 0 && v[e] > 0.0) cv[e] = 1;
-          }
+          const float g = (float)x.gv[e] * gs;
+          x.mv[e] = x.mv[e] * b1 + g * omb1;
+          x.vv[e] = x.vv[e] * b2 + g * g * omb2;
         }
       } else {
-        msc = vsc = __builtin_nanf("");
+        const double ma = (double)x.ms * (a.beta1 / (127.0 * 127.0)), va = (double)x.vs * (a.beta2 / (255.0 * 255.0 * 255.0 * 255.0));
+        double m[4], v[4];
+        float mm = 0.f, vm = 0.f, bad = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const double g = (double)x.gv[e];
+          const int c = (int)(int8_t)(x.mc >> (8 * e));
+          const unsigned q = (unsigned)(x.vc >> (8 * e)) & 255u, q2 = q * q;              // < 2^16: its square fits 32 bits
+          m[e] = fma(g, k1, ma * (double)(c * abs(c)));
+          v[e] = fma(g * g, k2, va * (double)(q2 * q2));
+          x.mv[e] = (float)m[e];
+          x.vv[e] = (float)v[e];
+          bad = fmaf(x.mv[e], 0.f, fmaf(x.vv[e], 0.f, bad));             // NaN as soon as one is not finite
+          mm = fmaxf(mm, fabsf(x.mv[e]));                                // rounding keeps the order: the rounded maximum is the maximum rounded
+          vm = fmaxf(vm, x.vv[e]);
+        }
+        float msc = wave_max(mm), vsc = wave_max(vm);
+        unsigned mc = 0, vc = 0;
+        if (__any(bad != 0.f)) {
+          msc = vsc = __builtin_nanf("");
+        } else {
+          const float mi = __builtin_amdgcn_rcpf(msc), vi = __builtin_amdgcn_rcpf(vsc);       // not used below TINY
+          int cm[4], cv[4];
+          int near = (msc < TINY) | (vsc < TINY);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float tm = position<127, 2>(fabsf(x.mv[e]), mi), tv = position<255, 4>(x.vv[e], vi);
+            near |= (int)near_border(tm) | (int)near_border(tv);
+            cm[e] = min((int)(tm + 0.5f), 127);
+            cv[e] = min((int)(tv + 0.5f), 255);
+          }
+          if (__any(near)) {
+#pragma unroll 1
+            for (int e = 0; e < 4; ++e) {
+              const double me = e == 0 ? m[0] : e == 1 ? m[1] : e == 2 ? m[2] : m[3], ve = e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3];
+              const int c = msc > 0.f ? exact_code<127, 2>(fabs(me), (double)msc) : 0, w = vsc > 0.f ? exact_code<255, 4>(ve, (double)vsc) : 0;
+#pragma unroll
+              for (int f = 0; f < 4; ++f) { cm[f] = f == e ? c : cm[f]; cv[f] = f == e ? w : cv[f]; }
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            cm[e] = x.mv[e] < 0.f ? -cm[e] : cm[e];
+            cv[e] = vsc > 0.f && v[e] > 0.0 ? max(cv[e], 1) : cv[e];
+            mc |= (unsigned)(uint8_t)cm[e] << (8 * e);
+            vc |= (unsigned)cv[e] << (8 * e);
+          }
+        }
+        x.mc = (int)mc; x.vc = (int)vc; x.ms = msc; x.vs = vsc;
       }
-      *ms = make_char4((signed char)cm[0], (signed char)cm[1], (signed char)cm[2], (signed char)cm[3]);
-      *vs = make_uchar4((unsigned char)cv[0], (unsigned char)cv[1], (unsigned char)cv[2], (unsigned char)cv[3]);
-      if (lane == 0) { a.exp_avg_scale[blk] = msc; a.exp_avg_sq_scale[blk] = vsc; }
-    }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) pv[e] = pv[e] * shrink - lr1 * (mv[e] / (sqrtf(vv[e] * ic2) + eps));
-    if constexpr (sizeof(P) == 2) store_n<float, 4>(a.master + at, pv);
-    if constexpr (EMA) {
-      float ev[4];
-      load_n<float, 4>(a.ema + at, ev);
+      for (int e = 0; e < 4; ++e) {
+        // root and quotient to an ulp each, of an update that is itself a small part of the parameter; moments next to underflow are rooted 2^64 times as large
+        const float w = x.vv[e] * ic2;
+        const bool tiny = w < 0x1p-96f;
+        const float root = __builtin_amdgcn_sqrtf(tiny ? w * 0x1p64f : w), den = (tiny ? root * 0x1p-32f : root) + eps;
+        const float q = x.mv[e] * __builtin_amdgcn_rcpf(den);
+        x.pv[e] = fmaf(-lr1, q, x.pv[e] * shrink);
+      }
+      if constexpr (EMA) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) ev[e] = ev[e] * ema_d + pv[e] * ema_o;
-      store_n<float, 4>(a.ema + at, ev);
-    }
-    if (whole) {
-      store_n<P, 4>(p + lane * 4, pv);
-    } else {
+        for (int e = 0; e < 4; ++e) x.ev[e] = x.ev[e] * ema_d + x.pv[e] * ema_o;
+      }
+      // the next block's values are waited for here, before the stores: loads and stores share a counter, and a wait behind the stores would be one for them too
+      __builtin_amdgcn_s_waitcnt(0x0f70);                    // vmcnt(0)
+      if constexpr (BITS == 32) {
+        *(f4*)((float*)a.exp_avg + at) = x.mv;
+        *(f4*)((float*)a.exp_avg_sq + at) = x.vv;
+      } else {
+        *(int*)((int8_t*)a.exp_avg + at) = x.mc;
+        *(int*)((uint8_t*)a.exp_avg_sq + at) = x.vc;
+        if (lane == 0) { a.exp_avg_scale[blk] = x.ms; a.exp_avg_sq_scale[blk] = x.vs; }
+      }
+      if constexpr (sizeof(P) == 2) *(f4*)(a.master + at) = x.pv;
+      if constexpr (EMA) *(f4*)(a.ema + at) = x.ev;
+      float pv[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (lane * 4 + e < left) p[lane * 4 + e] = (P)pv[e];
+      for (int e = 0; e < 4; ++e) pv[e] = x.pv[e];
+      if (x.whole) {
+        store_n<P, 4>(p + lane * 4, pv);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (lane * 4 + e < x.b.left) p[lane * 4 + e] = (P)pv[e];
+      }
     }
+    x = next;
   }
   if (!a.last) return;
   // Every wave of this workgroup has read the counter (its products p1 and p2 are there); the last workgroup to say so moves it on and leaves the ticket
@@ -190,7 +267,9 @@ __global__ __launch_bounds__(256) void moments_kernel(const int8_t* __restrict__
 
 template <typename P, typename G, int BITS>
 void launch(const DptAdamWArgs& a, const Grads& g, hipStream_t st) {
-  const int need = (a.n_blocks + WAVES - 1) / WAVES, blocks = need < 1 ? 1 : need < 2048 ? need : 2048;
+  // at most one generation of resident workgroups: each of them pays the counter's atomic once
+  constexpr int MOST = 1536;
+  const int need = (a.n_blocks + WAVES - 1) / WAVES, blocks = need < 1 ? 1 : need < MOST ? need : MOST;
   if (a.ema) hipLaunchKernelGGL((step_kernel<P, G, BITS, true>), dim3(blocks), dim3(64 * WAVES), 0, st, a, g);
   else hipLaunchKernelGGL((step_kernel<P, G, BITS, false>), dim3(blocks), dim3(64 * WAVES), 0, st, a, g);
 }
@@ -209,7 +288,7 @@ int dpt_adamw_step(const DptAdamWArgs* a, const void* const* grads, void* stream
   if ((a->state_bits != 8 && a->state_bits != 32) || !a->counter) return DPT_E_BADARG;
   if (a->type != DPT_F32 && a->type != DPT_BF16) return DPT_E_BADARG;
   if (a->grad_type != a->type && a->grad_type != DPT_F32) return DPT_E_UNSUPPORTED;
-  if (a->n_blocks > 0 && (!a->block_tensor || !a->first_block || !a->numel || !a->param || !a->decay || !a->exp_avg || !a->exp_avg_sq ||
+  if (a->n_blocks > 0 && (!a->blocks || !a->exp_avg || !a->exp_avg_sq ||
                           (a->type == DPT_BF16 && !a->master) || (a->state_bits == 8 && (!a->exp_avg_scale || !a->exp_avg_sq_scale)))) return DPT_E_BADARG;
   dpta::Grads g{};
   for (int i = 0; i < a->n_tensors; ++i) g.p[i] = grads[i];

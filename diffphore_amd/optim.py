@@ -20,6 +20,7 @@ from ._trainlib import TYPES, DptAdamWArgs, call, need_gpu
 BLOCK = 256                # elements of a tensor that share one scale of an 8-bit state; every tensor's slot in the flat buffers is a multiple of it
 _MAX_TENSORS = 400         # per launch
 _DTYPE = attrgetter("dtype")
+_RECORD = np.dtype([("param", "u8"), ("tensor", "i4"), ("index", "i4"), ("left", "i4"), ("decay", "f4"), ("pad", "i4", 2)])
 
 
 class AdamW:
@@ -65,25 +66,28 @@ class AdamW:
         self.params = params
         self._alias = [p.detach() for p in params]                       # keeps the updated memory alive whatever happens to the tensors
         self.dtype, self.device = params[0].dtype, params[0].device
-        index = {n: i for i, n in enumerate(self.names)} if self.names is not None else None
+        number = {n: i for i, n in enumerate(self.names)} if self.names is not None else None
         decay = np.ones(len(params), dtype=np.float32)
         for n in no_decay:
-            if (n not in index) if index is not None else not 0 <= int(n) < len(params):
+            if (n not in number) if number is not None else not 0 <= int(n) < len(params):
                 raise ValueError(f"no_decay: there is no parameter {n!r}")
-            decay[index[n] if index is not None else int(n)] = 0.0
+            decay[number[n] if number is not None else int(n)] = 0.0
         self._numel, self._sizes = [p.numel() for p in params], [p.shape for p in params]
         blocks = [-(-n // BLOCK) for n in self._numel]
         self.first_block = [0]
         for b in blocks:
             self.first_block.append(self.first_block[-1] + b)
         self.n_blocks = self.first_block[-1]
-        if self.n_blocks >= 1 << 31:
+        if self.n_blocks >= 1 << 30:
             raise ValueError("too many elements")
 
-        def up(x, dtype):
-            return torch.as_tensor(np.asarray(x, dtype=dtype)).to(self.device)
-        self._tables = {"block_tensor": up(np.repeat(np.arange(len(params)), blocks), np.int32), "first_block": up(self.first_block, np.int32),
-                        "numel": up(self._numel, np.int64), "param": up([p.data_ptr() for p in params], np.int64), "decay": up(decay, np.float32)}
+        which = np.repeat(np.arange(len(params), dtype=np.int32), blocks)                # DptAdamWBlock records
+        index = np.arange(self.n_blocks, dtype=np.int32) - np.asarray(self.first_block[:-1], dtype=np.int32)[which]
+        rec = np.zeros(self.n_blocks, dtype=_RECORD)
+        rec["tensor"], rec["index"], rec["decay"] = which, index, decay[which]
+        rec["param"] = np.asarray([p.data_ptr() for p in params], dtype=np.uint64)[which] + index.astype(np.uint64) * (BLOCK * params[0].element_size())
+        rec["left"] = np.minimum(np.asarray(self._numel, dtype=np.int64)[which] - index.astype(np.int64) * BLOCK, BLOCK)
+        self._blocks = torch.from_numpy(rec.view(np.uint8)).to(self.device)
 
         def flat(dtype=torch.float32):
             return torch.zeros(self.n_blocks * BLOCK, dtype=dtype, device=self.device)
@@ -150,8 +154,7 @@ class AdamW:
         a = DptAdamWArgs()
         a.type, a.state_bits = TYPES[self.dtype], self.state_bits
         a.beta1, a.beta2, a.eps, a.weight_decay, a.ema_decay = *self.betas, self.eps, self.weight_decay, self.ema_decay or 0.0
-        for n, t in self._tables.items():
-            setattr(a, n, t.data_ptr())
+        a.blocks = self._blocks.data_ptr()
         for n in self._STATE:
             setattr(a, n, getattr(self, n).data_ptr() if getattr(self, n) is not None else None)
         a.counter = self._counter.data_ptr()

@@ -91,6 +91,15 @@ int dpt_attn_bwd(const DptAttnArgs* a, void* stream);
 #define DPT_ADAMW_BLOCK 256
 #define DPT_ADAMW_MAX_TENSORS 400  /* tensors per call; the host splits longer lists (`last` on the last call of a step) */
 
+/* where a block's elements are; one record per block, held on the device */
+typedef struct DptAdamWBlock {
+  uint64_t param;                  /* address of the block's first parameter */
+  int32_t tensor, index;           /* its tensor, and its number inside it */
+  int32_t left;                    /* elements of the tensor from the block's first on, 256 at most */
+  float decay;                     /* factor of weight_decay: 1 or 0 */
+  int32_t pad_[2];
+} DptAdamWBlock;
+
 typedef struct DptAdamWArgs {
   int32_t type, grad_type;         /* fp32/fp32, bf16/bf16 or bf16/fp32 */
   int32_t state_bits;              /* 8 or 32 */
@@ -100,12 +109,8 @@ typedef struct DptAdamWArgs {
   double lr, beta1, beta2, eps, weight_decay, ema_decay;
   const float* lr_dev;             /* NULL, or the learning rate (then `lr` is not read) */
   const float* grad_scale;         /* NULL, or the factor of the gradients */
-  const int32_t* block_tensor;     /* [all blocks] tensor of a block, counted from this call's first tensor's number tensor0 */
-  int32_t tensor0, pad_;
-  const int32_t* first_block;      /* [all tensors + 1] */
-  const int64_t* numel;            /* [all tensors] */
-  void* const* param;              /* [all tensors] device pointers, held on the device */
-  const float* decay;              /* [all tensors] factor of weight_decay: 1 or 0 */
+  const DptAdamWBlock* blocks;     /* [all blocks] */
+  int32_t tensor0, pad_;           /* this call's first tensor */
   float* master;                   /* bf16: [all blocks * 256] */
   float* ema;                      /* NULL or [all blocks * 256] */
   void *exp_avg, *exp_avg_sq;      /* [all blocks * 256] fp32, or int8 / uint8 */
