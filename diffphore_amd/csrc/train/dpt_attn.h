@@ -57,19 +57,19 @@ __device__ __forceinline__ constexpr int sw(int row) {
   else return (((row >> 2) & 1) << 3) | (((row >> 3) & 1) << 2) | (row & 3);
 }
 
-// one chunk of a row in memory; what lies behind the row's dim elements is 0
-template <typename T>
-__device__ __forceinline__ typename Tr<T>::frag load_chunk(const T* __restrict__ row, int c, int dim, int vec) {
+// one chunk of a row in memory; what lies behind the row's dim elements is 0.  VEC: rows may be read 16 bytes at a time (dim is a multiple of a chunk)
+template <typename T, bool VEC>
+__device__ __forceinline__ typename Tr<T>::frag load_chunk(const T* __restrict__ row, int c, int dim) {
   constexpr int CH = Tr<T>::CH;
   typename Tr<T>::frag v;
-  if (vec) {
+  if constexpr (VEC) {
     if (c * CH < dim) return *reinterpret_cast<const typename Tr<T>::frag*>(row + c * CH);
 #pragma unroll
     for (int e = 0; e < CH; ++e) v[e] = (T)0.f;
-    return v;
-  }
+  } else {
 #pragma unroll
-  for (int e = 0; e < CH; ++e) v[e] = c * CH + e < dim ? row[c * CH + e] : (T)0.f;
+    for (int e = 0; e < CH; ++e) v[e] = c * CH + e < dim ? row[c * CH + e] : (T)0.f;
+  }
   return v;
 }
 
@@ -136,8 +136,8 @@ __device__ __forceinline__ float half_max(float x) { return fmaxf(x, __shfl_xor(
 __device__ __forceinline__ float half_sum(float x) { return x + __shfl_xor(x, 32, 64); }
 
 // out[d = 32 dt + 8 g + 4 h + i] of the lane's column into a row of dim elements
-template <typename T, int DP>
-__device__ __forceinline__ void store_col(T* __restrict__ row, int h, int dim, int vec, const f16v* acc, float f) {
+template <typename T, int DP, bool VEC>
+__device__ __forceinline__ void store_col(T* __restrict__ row, int h, int dim, const f16v* acc, float f) {
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
@@ -146,7 +146,7 @@ __device__ __forceinline__ void store_col(T* __restrict__ row, int h, int dim, i
       float v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = acc[dt][4 * g + i] * f;
-      if (vec) {
+      if constexpr (VEC) {
         if (d < dim) store_n<T, 4>(row + d, v);
       } else {
 #pragma unroll
@@ -158,30 +158,30 @@ __device__ __forceinline__ void store_col(T* __restrict__ row, int h, int dim, i
 
 // A tile of ROWS rows is filled by the workgroup's NT lanes, 16 bytes per lane and turn, in LDS order: turn n of lane t fills chunk n NT + t, so the
 // lane's source is the chunk that the permutation puts there.  `at(row)` gives a row's address.
-//   vec: straight into LDS (no registers; the tile is there after the next __syncthreads, which waits for memory).  Chunks behind dim are not
+//   VEC: straight into LDS (no registers; the tile is there after the next __syncthreads, which waits for memory).  Chunks behind dim are not
 //        fetched: they hold the zeros that zero_pad() put there before the loop.
 //   otherwise: through registers, element by element.
-template <typename T, int DP, int ROWS, int NT, typename At>
-__device__ __forceinline__ void stage(T* tile, int dim, int vec, At at) {
+template <typename T, int DP, int ROWS, int NT, bool VEC, typename At>
+__device__ __forceinline__ void stage(T* tile, int dim, At at) {
   constexpr int N = NC<T, DP>, CH = Tr<T>::CH, TURNS = ROWS * N / NT;
   static_assert(ROWS * N % NT == 0, "every lane in every turn");
 #pragma unroll
   for (int n = 0; n < TURNS; ++n) {
     const int i = n * NT + threadIdx.x, row = i / N, c = (i % N) ^ sw<N>(row);
-    if (vec) {
+    if constexpr (VEC) {
       T* dst = tile + (n * NT + __builtin_amdgcn_readfirstlane(threadIdx.x & ~63)) * CH;
       if (c * CH < dim)
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(at(row) + c * CH),
                                          (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
     } else {
-      *reinterpret_cast<typename Tr<T>::frag*>(tile + i * CH) = load_chunk<T>(at(row), c, dim, 0);
+      *reinterpret_cast<typename Tr<T>::frag*>(tile + i * CH) = load_chunk<T, false>(at(row), c, dim);
     }
   }
 }
-template <typename T, int DP, int ROWS, int NT>
+template <typename T, int DP, int ROWS, int NT, bool VEC>
 __device__ __forceinline__ void zero_pad(T* tile, int dim) {
   constexpr int N = NC<T, DP>, CH = Tr<T>::CH;
-  if (dim == DP) return;
+  if (!VEC || dim == DP) return;
   for (int i = threadIdx.x; i < ROWS * N; i += NT) {
     const int row = i / N, c = (i % N) ^ sw<N>(row);
     typename Tr<T>::frag z;
@@ -191,10 +191,11 @@ __device__ __forceinline__ void zero_pad(T* tile, int dim) {
   }
 }
 
-// dpt_attn_f32.hip / dpt_attn_bf16.hip
-hipError_t fwd_f32(const Dev& d, bool small, hipStream_t st);
-hipError_t fwd_bf16(const Dev& d, bool small, hipStream_t st);
-hipError_t bwd_f32(const Dev& d, bool small_rows, bool small_keys, hipStream_t st);
-hipError_t bwd_bf16(const Dev& d, bool small_rows, bool small_keys, hipStream_t st);
+// dpt_attn_<type>_<padded head dimension>.hip
+#define DPT_ATTN_DECL(x)                                          \
+  hipError_t fwd_##x(const Dev& d, bool small, hipStream_t st);   \
+  hipError_t bwd_##x(const Dev& d, bool small_rows, bool small_keys, hipStream_t st);
+DPT_ATTN_DECL(f32_32) DPT_ATTN_DECL(f32_64) DPT_ATTN_DECL(f32_128) DPT_ATTN_DECL(bf16_32) DPT_ATTN_DECL(bf16_64) DPT_ATTN_DECL(bf16_128)
+#undef DPT_ATTN_DECL
 
 }  // namespace dptat

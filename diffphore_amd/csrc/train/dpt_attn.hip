@@ -49,9 +49,8 @@ Ws layout(const DptAttnArgs* a, bool backward, int splits) {
 
 // 16-byte reads of rows of q, k, v, dout and out, 16- or 8-byte stores: the row length, every stride and every address have to allow them
 bool vec(const DptAttnArgs* a, bool backward) {
-  const int n = a->type == DPT_F32 ? 4 : 8, size = 16 / n;
+  const int n = a->type == DPT_F32 ? 4 : 8;
   auto ok = [&](const void* p, int64_t r, int64_t h) { return (uintptr_t)p % 16 == 0 && r % n == 0 && h % n == 0; };
-  (void)size;
   bool v = a->dim % n == 0 && ok(a->q, a->q_row, a->q_head) && ok(a->k, a->k_row, a->k_head) && ok(a->v, a->v_row, a->v_head) && ok(a->out, 0, 0);
   if (backward) v = v && ok(a->dout, a->dout_row, a->dout_head) && ok(a->dq, 0, 0) && ok(a->dk, 0, 0) && ok(a->dv, 0, 0);
   return v;
@@ -66,6 +65,10 @@ Dev dev(const DptAttnArgs* a, bool backward) {
   d.splits = 1;
   return d;
 }
+
+// kernels by the head dimension, padded to 32, 64 or 128
+template <typename F>
+F pick(int dim, F f32, F f64, F f128) { return dim <= 32 ? f32 : dim <= 64 ? f64 : f128; }
 
 bool strides_bad(const DptAttnArgs* a) {
   return a->q_row < 0 || a->q_head < 0 || a->k_row < 0 || a->k_head < 0 || a->v_row < 0 || a->v_head < 0 || a->bias_head < 0 || a->bias_pair < 0;
@@ -102,7 +105,8 @@ int dpt_attn_fwd(const DptAttnArgs* a, void* stream) {
   const bool small = dptat::small_rows(a);
   const int bm = small ? 32 : 128;
   d.tiles = (int)(((int64_t)a->max_nq * d.group + bm - 1) / bm);
-  return (int)(a->type == DPT_F32 ? dptat::fwd_f32(d, small, (hipStream_t)stream) : dptat::fwd_bf16(d, small, (hipStream_t)stream));
+  using namespace dptat;
+  return (int)(a->type == DPT_F32 ? pick(a->dim, fwd_f32_32, fwd_f32_64, fwd_f32_128) : pick(a->dim, fwd_bf16_32, fwd_bf16_64, fwd_bf16_128))(d, small, (hipStream_t)stream);
 }
 
 int dpt_attn_bwd(const DptAttnArgs* a, void* stream) {
@@ -119,7 +123,8 @@ int dpt_attn_bwd(const DptAttnArgs* a, void* stream) {
   d.fac0 = (float*)((char*)a->ws + w.delta);
   d.fac1 = (float*)((char*)a->ws + 2 * w.delta);
   const bool sr = dptat::small_rows(a), sk = a->max_nk <= 64;
-  return (int)(a->type == DPT_F32 ? dptat::bwd_f32(d, sr, sk, (hipStream_t)stream) : dptat::bwd_bf16(d, sr, sk, (hipStream_t)stream));
+  using namespace dptat;
+  return (int)(a->type == DPT_F32 ? pick(a->dim, bwd_f32_32, bwd_f32_64, bwd_f32_128) : pick(a->dim, bwd_bf16_32, bwd_bf16_64, bwd_bf16_128))(d, sr, sk, (hipStream_t)stream);
 }
 
 }  // extern "C"

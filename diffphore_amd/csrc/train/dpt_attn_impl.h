@@ -97,7 +97,7 @@ __device__ __forceinline__ void zero(f16v* x) {
 // NW waves x 32 rows; keys in tiles of BN, the next tile on its way into the other LDS buffer while one is worked on.  One pass over the keys with a
 // running base and sum per row.  The base follows the row's maximum only when that has moved by more than 2^8 (exp of the difference then still has all its
 // bits, and so has a bf16 of it), so the accumulators are rescaled a few times per row instead of once per tile.
-template <typename T, int DP, int NW, int BN, bool BIAS>
+template <typename T, int DP, int NW, int BN, bool BIAS, bool VEC>
 __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void fwd_kernel(Dev d) {
   __shared__ __attribute__((aligned(16))) T kt0[BN * DP], vt0[BN * DP], kt1[BN * DP], vt1[BN * DP];
   constexpr int NT = 64 * NW, BM = 32 * NW, J = BN / 32;
@@ -118,19 +118,19 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void fwd_kernel(D
   const T* vb = (const T*)d.a.v + (int64_t)p.k0 * d.a.v_row + p.hk * d.a.v_head;
   // keys from the last one on repeat it: their scores are masked, and it brings in no value that the result does not hold anyway
   auto fetch = [&](T* kt, T* vt, int t) __attribute__((always_inline)) {
-    stage<T, DP, BN, NT>(kt, d.a.dim, d.vec, [&](int r) { return kb + (int64_t)min(t * BN + r, p.nk - 1) * d.a.k_row; });
-    stage<T, DP, BN, NT>(vt, d.a.dim, d.vec, [&](int r) { return vb + (int64_t)min(t * BN + r, p.nk - 1) * d.a.v_row; });
+    stage<T, DP, BN, NT, VEC>(kt, d.a.dim, [&](int r) { return kb + (int64_t)min(t * BN + r, p.nk - 1) * d.a.k_row; });
+    stage<T, DP, BN, NT, VEC>(vt, d.a.dim, [&](int r) { return vb + (int64_t)min(t * BN + r, p.nk - 1) * d.a.v_row; });
   };
   if (t0 < t1) fetch(kt0, vt0, t0);
-  zero_pad<T, DP, BN, NT>(kt0, d.a.dim);
-  zero_pad<T, DP, BN, NT>(vt0, d.a.dim);
-  zero_pad<T, DP, BN, NT>(kt1, d.a.dim);
-  zero_pad<T, DP, BN, NT>(vt1, d.a.dim);
+  zero_pad<T, DP, BN, NT, VEC>(kt0, d.a.dim);
+  zero_pad<T, DP, BN, NT, VEC>(vt0, d.a.dim);
+  zero_pad<T, DP, BN, NT, VEC>(kt1, d.a.dim);
+  zero_pad<T, DP, BN, NT, VEC>(vt1, d.a.dim);
   typename Tr<T>::frag qf[NC<T, DP> / 2];
   {
     const T* q = (const T*)d.a.q + row.token * d.a.q_row + row.head * d.a.q_head;
 #pragma unroll
-    for (int s = 0; s < NC<T, DP> / 2; ++s) qf[s] = load_chunk<T>(q, 2 * s + h, d.a.dim, d.vec);
+    for (int s = 0; s < NC<T, DP> / 2; ++s) qf[s] = load_chunk<T, VEC>(q, 2 * s + h, d.a.dim);
   }
   const T* bias = BIAS ? (const T*)d.a.bias + row.head * d.a.bias_head + (p.pair0 + (int64_t)row.i * p.nk) * d.a.bias_pair : nullptr;
   const float c = FAST<T, BIAS> ? d.a.scale * LOG2E : LOG2E;   // exp(s - base) = exp2((x - base) c)
@@ -189,11 +189,11 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void fwd_kernel(D
   const float lm = m == NEG_INF ? 0.f : l * __builtin_amdgcn_exp2f((base - m) * c), mm = FAST<T, BIAS> ? m * d.a.scale : m;
   const int64_t at = row.token * d.a.heads + row.head, st = (int64_t)row.head * d.a.n_q + row.token, plane = (int64_t)d.a.heads * d.a.n_q;
   if (d.splits == 1) {
-    store_col<T, DP>((T*)d.a.out + at * d.a.dim, h, d.a.dim, d.vec, o, l == 0.f ? 0.f : 1.f / l);
+    store_col<T, DP, VEC>((T*)d.a.out + at * d.a.dim, h, d.a.dim, o, l == 0.f ? 0.f : 1.f / l);
     if (h == 0) { d.a.stats[st] = mm; d.a.stats[plane + st] = lm; }
   } else {
     const float f = m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((base - m) * c);
-    store_col<float, DP>(d.part_o + (split * plane + at) * d.a.dim, h, d.a.dim, d.a.dim % 4 == 0, o, f);
+    store_col<float, DP, VEC>(d.part_o + (split * plane + at) * d.a.dim, h, d.a.dim, o, f);
     if (h == 0) { d.part_ml[2 * split * plane + st] = mm; d.part_ml[(2 * split + 1) * plane + st] = lm; }
   }
 }
@@ -246,7 +246,7 @@ struct Probs {
 // As the forward pass, with the probabilities formed again from the stored statistics: ds = p (do.v - delta), dq += ds k.  Writes delta = sum_d do o and the
 // rows' factors for the second kernel.  Where a complex's keys are one tile, delta is taken as sum_j p_j do.v_j instead: the stored out is rounded to
 // its type, and with few keys that rounding does not average out.
-template <typename T, int DP, int NW, int BN, bool BIAS>
+template <typename T, int DP, int NW, int BN, bool BIAS, bool VEC>
 __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dq_kernel(Dev d) {
   __shared__ __attribute__((aligned(16))) T kt0[BN * DP], vt0[BN * DP], kt1[BN * DP], vt1[BN * DP];
   constexpr int NT = 64 * NW, BM = 32 * NW, J = BN / 32;
@@ -264,14 +264,14 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dq_kernel(De
   const T* kb = (const T*)d.a.k + (int64_t)p.k0 * d.a.k_row + p.hk * d.a.k_head;
   const T* vb = (const T*)d.a.v + (int64_t)p.k0 * d.a.v_row + p.hk * d.a.v_head;
   auto fetch = [&](T* kt, T* vt, int t) __attribute__((always_inline)) {
-    stage<T, DP, BN, NT>(kt, d.a.dim, d.vec, [&](int r) { return kb + (int64_t)min(t * BN + r, p.nk - 1) * d.a.k_row; });
-    stage<T, DP, BN, NT>(vt, d.a.dim, d.vec, [&](int r) { return vb + (int64_t)min(t * BN + r, p.nk - 1) * d.a.v_row; });
+    stage<T, DP, BN, NT, VEC>(kt, d.a.dim, [&](int r) { return kb + (int64_t)min(t * BN + r, p.nk - 1) * d.a.k_row; });
+    stage<T, DP, BN, NT, VEC>(vt, d.a.dim, [&](int r) { return vb + (int64_t)min(t * BN + r, p.nk - 1) * d.a.v_row; });
   };
   if (ktiles) fetch(kt0, vt0, 0);
-  zero_pad<T, DP, BN, NT>(kt0, d.a.dim);
-  zero_pad<T, DP, BN, NT>(vt0, d.a.dim);
-  zero_pad<T, DP, BN, NT>(kt1, d.a.dim);
-  zero_pad<T, DP, BN, NT>(vt1, d.a.dim);
+  zero_pad<T, DP, BN, NT, VEC>(kt0, d.a.dim);
+  zero_pad<T, DP, BN, NT, VEC>(vt0, d.a.dim);
+  zero_pad<T, DP, BN, NT, VEC>(kt1, d.a.dim);
+  zero_pad<T, DP, BN, NT, VEC>(vt1, d.a.dim);
 
   const int64_t at = row.token * d.a.heads + row.head, st = (int64_t)row.head * d.a.n_q + row.token, plane = (int64_t)d.a.heads * d.a.n_q;
   const bool one = p.nk <= BN;
@@ -283,13 +283,13 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dq_kernel(De
     const T* o = (const T*)d.a.out + at * d.a.dim;
 #pragma unroll
     for (int s = 0; s < NC<T, DP> / 2; ++s) {
-      qf[s] = load_chunk<T>(q, 2 * s + h, d.a.dim, d.vec);
-      gf[s] = load_chunk<T>(g, 2 * s + h, d.a.dim, d.vec);
+      qf[s] = load_chunk<T, VEC>(q, 2 * s + h, d.a.dim);
+      gf[s] = load_chunk<T, VEC>(g, 2 * s + h, d.a.dim);
     }
     if (!one) {
 #pragma unroll
       for (int s = 0; s < NC<T, DP> / 2; ++s) {
-        const typename Tr<T>::frag of = load_chunk<T>(o, 2 * s + h, d.a.dim, d.vec);
+        const typename Tr<T>::frag of = load_chunk<T, VEC>(o, 2 * s + h, d.a.dim);
 #pragma unroll
         for (int e = 0; e < Tr<T>::CH; ++e) delta = fmaf((float)gf[s][e], (float)of[e], delta);
       }
@@ -358,7 +358,7 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dq_kernel(De
     work(kt1, vt1, t + 1);
   }
   if (!rb.live) return;
-  store_col<T, DP>((T*)d.a.dq + at * d.a.dim, h, d.a.dim, d.vec, dq, d.a.scale);
+  store_col<T, DP, VEC>((T*)d.a.dq + at * d.a.dim, h, d.a.dim, dq, d.a.scale);
   if (h == 0) {
     d.delta[st] = delta;
     d.fac0[st] = f.f0;
@@ -376,8 +376,8 @@ struct RowTile {
   int64_t bias[BIAS ? BR : 1];
 };
 
-template <typename T, int DP, int NW, int BR, bool BIAS>
-__global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dkv_kernel(Dev d) {
+template <typename T, int DP, int NW, int BR, bool BIAS, bool VEC>
+__global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> && DP <= 64 ? 2 : 1)) void dkv_kernel(Dev d) {
   __shared__ RowTile<T, DP, NW, BR, BIAS> rt0, rt1;
   constexpr int NT = 64 * NW, BM = 32 * NW, J = BR / 32;
   const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
@@ -394,8 +394,8 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dkv_kernel(D
 
   auto fetch = [&](RowTile<T, DP, NW, BR, BIAS>& rt, int t) __attribute__((always_inline)) {
     auto src = [&](int r) __attribute__((always_inline)) { return row_at(d, p, min(t * BR + r, p.rows - 1)); };
-    stage<T, DP, BR, NT>(rt.q, d.a.dim, d.vec, [&](int r) { const Row x = src(r); return (const T*)d.a.q + x.token * d.a.q_row + x.head * d.a.q_head; });
-    stage<T, DP, BR, NT>(rt.g, d.a.dim, d.vec, [&](int r) { const Row x = src(r); return (const T*)d.a.dout + x.token * d.a.dout_row + x.head * d.a.dout_head; });
+    stage<T, DP, BR, NT, VEC>(rt.q, d.a.dim, [&](int r) { const Row x = src(r); return (const T*)d.a.q + x.token * d.a.q_row + x.head * d.a.q_head; });
+    stage<T, DP, BR, NT, VEC>(rt.g, d.a.dim, [&](int r) { const Row x = src(r); return (const T*)d.a.dout + x.token * d.a.dout_row + x.head * d.a.dout_head; });
     if (threadIdx.x < BR) {
       const Row x = src(threadIdx.x);
       const int64_t st = (int64_t)x.head * d.a.n_q + x.token;
@@ -406,16 +406,16 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dkv_kernel(D
     }
   };
   if (first < last) fetch(rt0, first);
-  zero_pad<T, DP, BR, NT>(rt0.q, d.a.dim);
-  zero_pad<T, DP, BR, NT>(rt0.g, d.a.dim);
-  zero_pad<T, DP, BR, NT>(rt1.q, d.a.dim);
-  zero_pad<T, DP, BR, NT>(rt1.g, d.a.dim);
+  zero_pad<T, DP, BR, NT, VEC>(rt0.q, d.a.dim);
+  zero_pad<T, DP, BR, NT, VEC>(rt0.g, d.a.dim);
+  zero_pad<T, DP, BR, NT, VEC>(rt1.q, d.a.dim);
+  zero_pad<T, DP, BR, NT, VEC>(rt1.g, d.a.dim);
 
   typename Tr<T>::frag kf[NC<T, DP> / 2], vf[NC<T, DP> / 2];
 #pragma unroll
   for (int s = 0; s < NC<T, DP> / 2; ++s) {
-    kf[s] = load_chunk<T>((const T*)d.a.k + token * d.a.k_row + p.hk * d.a.k_head, 2 * s + h, d.a.dim, d.vec);
-    vf[s] = load_chunk<T>((const T*)d.a.v + token * d.a.v_row + p.hk * d.a.v_head, 2 * s + h, d.a.dim, d.vec);
+    kf[s] = load_chunk<T, VEC>((const T*)d.a.k + token * d.a.k_row + p.hk * d.a.k_head, 2 * s + h, d.a.dim);
+    vf[s] = load_chunk<T, VEC>((const T*)d.a.v + token * d.a.v_row + p.hk * d.a.v_head, 2 * s + h, d.a.dim);
   }
   const float c = FAST<T, BIAS> ? d.a.scale * LOG2E : LOG2E;
   f16v dk[DP / 32], dv[DP / 32];
@@ -471,30 +471,24 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dkv_kernel(D
   }
   if (live) {
     const int64_t at = (token * d.a.kv_heads + p.hk) * d.a.dim;
-    store_col<T, DP>((T*)d.a.dk + at, h, d.a.dim, d.vec, dk, d.a.scale);
-    store_col<T, DP>((T*)d.a.dv + at, h, d.a.dim, d.vec, dv, 1.f);
+    store_col<T, DP, VEC>((T*)d.a.dk + at, h, d.a.dim, dk, d.a.scale);
+    store_col<T, DP, VEC>((T*)d.a.dv + at, h, d.a.dim, dv, 1.f);
   }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool BIAS, bool VEC>
 hipError_t run_fwd(const Dev& d, bool small, hipStream_t st) {
   constexpr int BN = sizeof(T) == 2 ? 64 : 32;
   const unsigned n = (unsigned)((int64_t)d.tiles * d.a.B * d.a.kv_heads * d.splits);
   if (n) {
-    if (d.a.bias) {
-      if (small) hipLaunchKernelGGL((fwd_kernel<T, DP, 1, BN, true>), dim3(n), dim3(64), 0, st, d);
-      else hipLaunchKernelGGL((fwd_kernel<T, DP, 4, BN, true>), dim3(n), dim3(256), 0, st, d);
-    } else {
-      if (small) hipLaunchKernelGGL((fwd_kernel<T, DP, 1, BN, false>), dim3(n), dim3(64), 0, st, d);
-      else hipLaunchKernelGGL((fwd_kernel<T, DP, 4, BN, false>), dim3(n), dim3(256), 0, st, d);
-    }
-    if (d.splits > 1)
-      hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(((int64_t)d.a.heads * d.a.n_q + 3) / 4)), dim3(256), 0, st, d);
+    if (small) hipLaunchKernelGGL((fwd_kernel<T, DP, 1, BN, BIAS, VEC>), dim3(n), dim3(64), 0, st, d);
+    else hipLaunchKernelGGL((fwd_kernel<T, DP, 4, BN, BIAS, VEC>), dim3(n), dim3(256), 0, st, d);
+    if (d.splits > 1) hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(((int64_t)d.a.heads * d.a.n_q + 3) / 4)), dim3(256), 0, st, d);
   }
   return hipGetLastError();
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool BIAS, bool VEC>
 hipError_t run_bwd(const Dev& d0, bool small_rows, bool small_keys, hipStream_t st) {
   constexpr int BN = sizeof(T) == 2 ? 64 : 32, BR = BN;
   Dev d = d0;
@@ -502,35 +496,27 @@ hipError_t run_bwd(const Dev& d0, bool small_rows, bool small_keys, hipStream_t 
   d.tiles = (int)((rows + (small_rows ? 31 : 127)) / (small_rows ? 32 : 128));
   const unsigned n = (unsigned)((int64_t)d.tiles * d.a.B * d.a.kv_heads);
   if (n) {
-    if (d.a.bias) {
-      if (small_rows) hipLaunchKernelGGL((dq_kernel<T, DP, 1, BN, true>), dim3(n), dim3(64), 0, st, d);
-      else hipLaunchKernelGGL((dq_kernel<T, DP, 4, BN, true>), dim3(n), dim3(256), 0, st, d);
-    } else {
-      if (small_rows) hipLaunchKernelGGL((dq_kernel<T, DP, 1, BN, false>), dim3(n), dim3(64), 0, st, d);
-      else hipLaunchKernelGGL((dq_kernel<T, DP, 4, BN, false>), dim3(n), dim3(256), 0, st, d);
-    }
+    if (small_rows) hipLaunchKernelGGL((dq_kernel<T, DP, 1, BN, BIAS, VEC>), dim3(n), dim3(64), 0, st, d);
+    else hipLaunchKernelGGL((dq_kernel<T, DP, 4, BN, BIAS, VEC>), dim3(n), dim3(256), 0, st, d);
   }
   d.tiles = (d.a.max_nk + (small_keys ? 31 : 127)) / (small_keys ? 32 : 128);
   const unsigned nk = (unsigned)((int64_t)d.tiles * d.a.B * d.a.kv_heads);
   if (nk) {
-    if (d.a.bias) {
-      if (small_keys) hipLaunchKernelGGL((dkv_kernel<T, DP, 1, BR, true>), dim3(nk), dim3(64), 0, st, d);
-      else hipLaunchKernelGGL((dkv_kernel<T, DP, 4, BR, true>), dim3(nk), dim3(256), 0, st, d);
-    } else {
-      if (small_keys) hipLaunchKernelGGL((dkv_kernel<T, DP, 1, BR, false>), dim3(nk), dim3(64), 0, st, d);
-      else hipLaunchKernelGGL((dkv_kernel<T, DP, 4, BR, false>), dim3(nk), dim3(256), 0, st, d);
-    }
+    if (small_keys) hipLaunchKernelGGL((dkv_kernel<T, DP, 1, BR, BIAS, VEC>), dim3(nk), dim3(64), 0, st, d);
+    else hipLaunchKernelGGL((dkv_kernel<T, DP, 4, BR, BIAS, VEC>), dim3(nk), dim3(256), 0, st, d);
   }
   return hipGetLastError();
 }
 
-template <typename T>
-hipError_t fwd_by_dim(const Dev& d, bool small, hipStream_t st) {
-  return d.a.dim <= 32 ? run_fwd<T, 32>(d, small, st) : d.a.dim <= 64 ? run_fwd<T, 64>(d, small, st) : run_fwd<T, 128>(d, small, st);
+template <typename T, int DP>
+hipError_t fwd_of(const Dev& d, bool small, hipStream_t st) {
+  if (d.a.bias) return d.vec ? run_fwd<T, DP, true, true>(d, small, st) : run_fwd<T, DP, true, false>(d, small, st);
+  return d.vec ? run_fwd<T, DP, false, true>(d, small, st) : run_fwd<T, DP, false, false>(d, small, st);
 }
-template <typename T>
-hipError_t bwd_by_dim(const Dev& d, bool sr, bool sk, hipStream_t st) {
-  return d.a.dim <= 32 ? run_bwd<T, 32>(d, sr, sk, st) : d.a.dim <= 64 ? run_bwd<T, 64>(d, sr, sk, st) : run_bwd<T, 128>(d, sr, sk, st);
+template <typename T, int DP>
+hipError_t bwd_of(const Dev& d, bool sr, bool sk, hipStream_t st) {
+  if (d.a.bias) return d.vec ? run_bwd<T, DP, true, true>(d, sr, sk, st) : run_bwd<T, DP, true, false>(d, sr, sk, st);
+  return d.vec ? run_bwd<T, DP, false, true>(d, sr, sk, st) : run_bwd<T, DP, false, false>(d, sr, sk, st);
 }
 
 }  // namespace dptat
