@@ -157,26 +157,40 @@ __device__ __forceinline__ void store_col(T* __restrict__ row, int h, int dim, c
 }
 
 // A tile of ROWS rows is filled by the workgroup's NT lanes, 16 bytes per lane and turn, in LDS order: turn n of lane t fills chunk n NT + t, so the
-// lane's source is the chunk that the permutation puts there.  `at(row)` gives a row's address.
-//   VEC: straight into LDS (no registers; the tile is there after the next __syncthreads, which waits for memory).  Chunks behind dim are not
+// lane's source is the chunk that the permutation puts there.
+//   VEC: straight into LDS (no registers; the tile is there after the next tile_barrier).  Chunks behind dim are not
 //        fetched: they hold the zeros that zero_pad() put there before the loop.
 //   otherwise: through registers, element by element.
-template <typename T, int DP, int ROWS, int NT, bool VEC, typename At>
-__device__ __forceinline__ void stage(T* tile, int dim, At at) {
-  constexpr int N = NC<T, DP>, CH = Tr<T>::CH, TURNS = ROWS * N / NT;
-  static_assert(ROWS * N % NT == 0, "every lane in every turn");
-#pragma unroll
-  for (int n = 0; n < TURNS; ++n) {
-    const int i = n * NT + threadIdx.x, row = i / N, c = (i % N) ^ sw<N>(row);
-    if constexpr (VEC) {
-      T* dst = tile + (n * NT + __builtin_amdgcn_readfirstlane(threadIdx.x & ~63)) * CH;
-      if (c * CH < dim)
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(at(row) + c * CH),
-                                         (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
-    } else {
-      *reinterpret_cast<typename Tr<T>::frag*>(tile + i * CH) = load_chunk<T, false>(at(row), c, dim);
-    }
+template <typename T, int DP, int NT, bool VEC>
+__device__ __forceinline__ void stage_chunk(T* tile, int n, int c, int dim, const T* row) {
+  constexpr int CH = Tr<T>::CH;
+  if constexpr (VEC) {
+    T* dst = tile + (n * NT + __builtin_amdgcn_readfirstlane(threadIdx.x & ~63)) * CH;
+    if (c * CH < dim)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(row + c * CH), (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+  } else {
+    *reinterpret_cast<typename Tr<T>::frag*>(tile + (n * NT + threadIdx.x) * CH) = load_chunk<T, false>(row, c, dim);
   }
+}
+// rows of a regular array, `there` of them (at least one): row r at src + r stride.  What follows the last one repeats it.
+// (VEC: the host has checked that a tile's offsets fit 32 bits; a 64-bit multiplication costs several times as much)
+template <typename T, int DP, int ROWS, int NT, bool VEC>
+__device__ __forceinline__ void stage(T* tile, int dim, const T* src, int64_t stride, int there) {
+  constexpr int N = NC<T, DP>, STEP = NT / N;
+  static_assert(NT % N == 0 && ROWS % STEP == 0, "every lane in every turn");
+#pragma unroll
+  for (int n = 0; n < ROWS / STEP; ++n) {
+    const int row = n * STEP + threadIdx.x / N, r = min(row, there - 1);
+    const T* p = VEC ? src + (uint32_t)r * (uint32_t)stride : src + (int64_t)r * stride;
+    stage_chunk<T, DP, NT, VEC>(tile, n, (threadIdx.x % N) ^ sw<N>(row), dim, p);
+  }
+}
+
+// The barrier between tiles: every wave waits for its own fetches into LDS, then for the others.  The wait is written out: the compiler orders a workgroup's
+// plain LDS accesses at a barrier, but does not hold a barrier back for fetches that go past the registers (seen in its output: none on a loop's way back).
+__device__ __forceinline__ void tile_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
 }
 template <typename T, int DP, int ROWS, int NT, bool VEC>
 __device__ __forceinline__ void zero_pad(T* tile, int dim) {

@@ -50,7 +50,8 @@ Ws layout(const DptAttnArgs* a, bool backward, int splits) {
 // 16-byte reads of rows of q, k, v, dout and out, 16- or 8-byte stores: the row length, every stride and every address have to allow them
 bool vec(const DptAttnArgs* a, bool backward) {
   const int n = a->type == DPT_F32 ? 4 : 8;
-  auto ok = [&](const void* p, int64_t r, int64_t h) { return (uintptr_t)p % 16 == 0 && r % n == 0 && h % n == 0; };
+  // (strides below 2^24: 64 rows and as many heads apart still fit the 32-bit offset that the kernels use)
+  auto ok = [&](const void* p, int64_t r, int64_t h) { return (uintptr_t)p % 16 == 0 && r % n == 0 && h % n == 0 && r < 1 << 24 && h < 1 << 24; };
   bool v = a->dim % n == 0 && ok(a->q, a->q_row, a->q_head) && ok(a->k, a->k_row, a->k_head) && ok(a->v, a->v_row, a->v_head) && ok(a->out, 0, 0);
   if (backward) v = v && ok(a->dout, a->dout_row, a->dout_head) && ok(a->dq, 0, 0) && ok(a->dk, 0, 0) && ok(a->dv, 0, 0);
   return v;

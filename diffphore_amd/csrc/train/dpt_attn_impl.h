@@ -116,10 +116,10 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void fwd_kernel(D
 
   const T* kb = (const T*)d.a.k + (int64_t)p.k0 * d.a.k_row + p.hk * d.a.k_head;
   const T* vb = (const T*)d.a.v + (int64_t)p.k0 * d.a.v_row + p.hk * d.a.v_head;
-  // keys from the last one on repeat it: their scores are masked, and it brings in no value that the result does not hold anyway
+  // keys behind the last one repeat it: their scores are masked, and it brings in no value that the result does not hold anyway
   auto fetch = [&](T* kt, T* vt, int t) __attribute__((always_inline)) {
-    stage<T, DP, BN, NT, VEC>(kt, d.a.dim, [&](int r) { return kb + (int64_t)min(t * BN + r, p.nk - 1) * d.a.k_row; });
-    stage<T, DP, BN, NT, VEC>(vt, d.a.dim, [&](int r) { return vb + (int64_t)min(t * BN + r, p.nk - 1) * d.a.v_row; });
+    stage<T, DP, BN, NT, VEC>(kt, d.a.dim, kb + (int64_t)t * BN * d.a.k_row, d.a.k_row, p.nk - t * BN);
+    stage<T, DP, BN, NT, VEC>(vt, d.a.dim, vb + (int64_t)t * BN * d.a.v_row, d.a.v_row, p.nk - t * BN);
   };
   if (t0 < t1) fetch(kt0, vt0, t0);
   zero_pad<T, DP, BN, NT, VEC>(kt0, d.a.dim);
@@ -175,11 +175,11 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void fwd_kernel(D
   };
   // one barrier per tile: it waits for the tile's fetch and for the last reads of the buffer that the next fetch overwrites
   for (int t = t0; t < t1; t += 2) {
-    __syncthreads();
+    tile_barrier();
     if (t + 1 < t1) fetch(kt1, vt1, t + 1);
     work(kt0, vt0, t);
     if (t + 1 >= t1) break;
-    __syncthreads();
+    tile_barrier();
     if (t + 2 < t1) fetch(kt0, vt0, t + 2);
     work(kt1, vt1, t + 1);
   }
@@ -264,8 +264,8 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dq_kernel(De
   const T* kb = (const T*)d.a.k + (int64_t)p.k0 * d.a.k_row + p.hk * d.a.k_head;
   const T* vb = (const T*)d.a.v + (int64_t)p.k0 * d.a.v_row + p.hk * d.a.v_head;
   auto fetch = [&](T* kt, T* vt, int t) __attribute__((always_inline)) {
-    stage<T, DP, BN, NT, VEC>(kt, d.a.dim, [&](int r) { return kb + (int64_t)min(t * BN + r, p.nk - 1) * d.a.k_row; });
-    stage<T, DP, BN, NT, VEC>(vt, d.a.dim, [&](int r) { return vb + (int64_t)min(t * BN + r, p.nk - 1) * d.a.v_row; });
+    stage<T, DP, BN, NT, VEC>(kt, d.a.dim, kb + (int64_t)t * BN * d.a.k_row, d.a.k_row, p.nk - t * BN);
+    stage<T, DP, BN, NT, VEC>(vt, d.a.dim, vb + (int64_t)t * BN * d.a.v_row, d.a.v_row, p.nk - t * BN);
   };
   if (ktiles) fetch(kt0, vt0, 0);
   zero_pad<T, DP, BN, NT, VEC>(kt0, d.a.dim);
@@ -349,11 +349,11 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dq_kernel(De
     }
   };
   for (int t = 0; t < ktiles; t += 2) {
-    __syncthreads();
+    tile_barrier();
     if (t + 1 < ktiles) fetch(kt1, vt1, t + 1);
     work(kt0, vt0, t);
     if (t + 1 >= ktiles) break;
-    __syncthreads();
+    tile_barrier();
     if (t + 2 < ktiles) fetch(kt0, vt0, t + 2);
     work(kt1, vt1, t + 1);
   }
@@ -392,10 +392,34 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> && DP <= 64 ? 2 : 1)) void 
   const int rmin = rows_from(key), r_lo = __builtin_amdgcn_readfirstlane(rows_from(w0)), r_hi = __builtin_amdgcn_readfirstlane(rows_from(w0 + 31));
   const int first = rows_from(key0) / BR, last = (p.rows + BR - 1) / BR;
 
+  const int li = div_group(d, threadIdx.x / NC<T, DP>), lg = threadIdx.x / NC<T, DP> - li * d.group;
+  const uint32_t q_off = (uint32_t)li * (uint32_t)d.a.q_row + (uint32_t)lg * (uint32_t)d.a.q_head, g_off = (uint32_t)li * (uint32_t)d.a.dout_row + (uint32_t)lg * (uint32_t)d.a.dout_head;
   auto fetch = [&](RowTile<T, DP, NW, BR, BIAS>& rt, int t) __attribute__((always_inline)) {
-    auto src = [&](int r) __attribute__((always_inline)) { return row_at(d, p, min(t * BR + r, p.rows - 1)); };
-    stage<T, DP, BR, NT, VEC>(rt.q, d.a.dim, [&](int r) { const Row x = src(r); return (const T*)d.a.q + x.token * d.a.q_row + x.head * d.a.q_head; });
-    stage<T, DP, BR, NT, VEC>(rt.g, d.a.dim, [&](int r) { const Row x = src(r); return (const T*)d.a.dout + x.token * d.a.dout_row + x.head * d.a.dout_head; });
+    const int r0 = t * BR;
+    auto src = [&](int r) __attribute__((always_inline)) { return row_at(d, p, min(r0 + r, p.rows - 1)); };
+    // as stage(): with 1, 2, 4 .. STEP heads in the group, rows STEP apart are the same head of queries STEP / group apart
+    constexpr int N = NC<T, DP>, STEP = NT / N;
+    const int row0 = threadIdx.x / N;
+    if (VEC && r0 + BR <= p.rows && STEP % d.group == 0) {
+      const int64_t i0 = p.q0 + r0 / d.group;
+      const T* q0 = (const T*)d.a.q + i0 * d.a.q_row + (int64_t)p.hk * d.group * d.a.q_head;
+      const T* g0 = (const T*)d.a.dout + i0 * d.a.dout_row + (int64_t)p.hk * d.group * d.a.dout_head;
+#pragma unroll
+      for (int n = 0; n < BR / STEP; ++n) {
+        const int c = (threadIdx.x % N) ^ sw<N>(n * STEP + row0);
+        const int64_t di = n * (STEP / d.group);
+        stage_chunk<T, DP, NT, VEC>(rt.q, n, c, d.a.dim, q0 + di * d.a.q_row + q_off);
+        stage_chunk<T, DP, NT, VEC>(rt.g, n, c, d.a.dim, g0 + di * d.a.dout_row + g_off);
+      }
+    } else {
+#pragma unroll 1
+      for (int n = 0; n < BR / STEP; ++n) {
+        const Row x = src(n * STEP + row0);
+        const int c = (threadIdx.x % N) ^ sw<N>(n * STEP + row0);
+        stage_chunk<T, DP, NT, VEC>(rt.q, n, c, d.a.dim, (const T*)d.a.q + x.token * d.a.q_row + x.head * d.a.q_head);
+        stage_chunk<T, DP, NT, VEC>(rt.g, n, c, d.a.dim, (const T*)d.a.dout + x.token * d.a.dout_row + x.head * d.a.dout_head);
+      }
+    }
     if (threadIdx.x < BR) {
       const Row x = src(threadIdx.x);
       const int64_t st = (int64_t)x.head * d.a.n_q + x.token;
@@ -461,11 +485,11 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> && DP <= 64 ? 2 : 1)) void 
     }
   };
   for (int t = first; t < last; t += 2) {
-    __syncthreads();
+    tile_barrier();
     if (t + 1 < last) fetch(rt1, t + 1);
     work(rt0, t);
     if (t + 1 >= last) break;
-    __syncthreads();
+    tile_barrier();
     if (t + 2 < last) fetch(rt0, t + 2);
     work(rt1, t + 1);
   }
