@@ -13,7 +13,7 @@ namespace dptn {
 using namespace dpt;
 
 constexpr int MAX_WIDTH = 16384;
-constexpr int PARTS = 512;           // most partial rows of the column sums
+constexpr int PARTS = 1024;           // most partial rows of the column sums
 
 // sum over the L lanes of a row; L > 64: over the workgroup (blockDim.x == L), through LDS.  N sums at a time.
 template <int L, int N>
@@ -121,44 +121,83 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void fwd_kernel(int64_t rows, in
   }
 }
 
+// a row's elements of a lane as they lie in memory
+template <typename T, int E, int V>
+struct Raw {
+  typedef __attribute__((ext_vector_type(V))) T vec;
+  vec v[E / V];
+  template <int L>
+  __device__ __forceinline__ void load(const T* __restrict__ p, int lane, int width) {
+#pragma unroll
+    for (int i = 0; i < E / V; ++i) {
+      const int c = column<L, V>(lane, i * V);
+      if (c < width) {
+        v[i] = *reinterpret_cast<const vec*>(p + c);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[i][e] = (T)0.f;
+      }
+    }
+  }
+  __device__ __forceinline__ float operator[](int e) const { return (float)v[e / V][e % V]; }
+};
+
+// One exchange per row: with u = x - mean (as stored) the three sums of u, g and g u give what the rounding of the stored mean left (c = mean u), mean g
+// and mean(g xh) = rstd (mean(g u) - c mean g).  The next row is on its way while a row is worked on, and the weight stays in registers (not in the widest
+// rows: 1024 lanes have 128 registers each).
 template <typename T, typename W, int L, int E, int V>
 __global__ __launch_bounds__(L > 256 ? L : 256) void bwd_kernel(int64_t rows, int width, const T* __restrict__ dy, int64_t dys, const T* __restrict__ x,
                                                                 int64_t xs, const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                 const W* __restrict__ w, T* __restrict__ dx, int64_t dxs, float* __restrict__ part) {
   constexpr int TPB = L > 256 ? L : 256, G = TPB / L;
-  __shared__ float red[L > 64 ? 2 * (L / 64) : 1];
+  constexpr bool ROOM = L < 1024;
+  __shared__ float red[L > 64 ? 3 * (L / 64) : 1];
   __shared__ float cols[G > 1 ? G * L * E : 1];
   const int lane = threadIdx.x % L;
   const int64_t groups = (int64_t)gridDim.x * G;
   const float inv = 1.f / (float)width;
-  // the weight stays in registers too, but for the widest rows, whose lanes have none left: there it is read again for each row (from cache)
-  constexpr bool KEEP_W = E <= 16;
   float wv[E], dw[E], db[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) { wv[e] = 1.f; dw[e] = 0.f; db[e] = 0.f; }
-  if (KEEP_W && w) load_row<W, L, E, V>(w, lane, width, wv);
-  for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < rows; r0 += groups) {
+  if (ROOM && w) load_row<W, L, E, V>(w, lane, width, wv);
+  Raw<T, E, V> xr, gr;
+  float mr, rr;
+  auto fetch = [&](int64_t r0) __attribute__((always_inline)) {
+    const int64_t r = r0 + threadIdx.x / L, at = r < rows ? r : rows - 1;
+    xr.template load<L>(x + at * xs, lane, width);
+    gr.template load<L>(dy + at * dys, lane, width);
+    mr = mean[at];
+    rr = rstd[at];
+  };
+  int64_t r0 = (int64_t)blockIdx.x * G;
+  if (ROOM && r0 < rows) fetch(r0);
+  for (; r0 < rows; r0 += groups) {
     const int64_t r = r0 + threadIdx.x / L;
     const bool live = r < rows;
-    const int64_t rr = live ? r : rows - 1;
-    float v[E], g[E], m, s[2] = {0.f, 0.f};
-    load_row<T, L, E, V>(x + rr * xs, lane, width, v);
-    load_row<T, L, E, V>(dy + rr * dys, lane, width, g);
-    const float rs = rstd[rr];
-    if (!KEEP_W && w) load_row<W, L, E, V>(w, lane, width, wv);
-    centre<L, E, V>(v, mean[rr], lane, width, inv, &m, red);
+    float v[E], g[E], s[3] = {0.f, 0.f, 0.f};
+    if constexpr (!ROOM) {
+      fetch(r0);
+      if (w) load_row<W, L, E, V>(w, lane, width, wv);
+    }
+    const float rs = rr;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      v[e] *= rs;
-      if (live) { dw[e] = fmaf(g[e], v[e], dw[e]); db[e] += g[e]; }
-      g[e] *= wv[e];
-      s[0] += g[e];
-      s[1] = fmaf(g[e], v[e], s[1]);
+      v[e] = column<L, V>(lane, e) < width ? xr[e] - mr : 0.f;
+      g[e] = gr[e];
+      const float t = g[e] * wv[e];
+      s[0] += v[e];
+      s[1] += t;
+      s[2] = fmaf(t, v[e], s[2]);
     }
-    row_sum<L, 2>(s, red);
-    const float a = s[0] * inv, c = s[1] * inv;
+    if (ROOM && r0 + groups < rows) fetch(r0 + groups);
+    row_sum<L, 3>(s, red);
+    const float c = s[0] * inv, a = s[1] * inv, q = rs * fmaf(-c, a, s[2] * inv);
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = rs * (g[e] - a - v[e] * c);
+    for (int e = 0; e < E; ++e) {
+      const float xh = (v[e] - c) * rs;
+      if (live) { dw[e] = fmaf(g[e], xh, dw[e]); db[e] += g[e]; }
+      v[e] = rs * (g[e] * wv[e] - a - xh * q);
+    }
     if (live) store_row<T, L, E, V>(dx + r * dxs, lane, width, v);
   }
   if (!part) return;
@@ -188,24 +227,24 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void bwd_kernel(int64_t rows, in
   }
 }
 
-// out[c] = sum over the partial rows, 8 strands of rows per column joined in order
+// out[c] = sum over the partial rows: 16 columns and 64 strands of rows per workgroup (16 loads one behind the other for the most partial rows), joined in order
 template <typename W>
-__global__ __launch_bounds__(256) void cols_kernel(int parts, int width, const float* __restrict__ part, W* __restrict__ dw, W* __restrict__ db) {
-  __shared__ float t[8][33];
-  const int c = blockIdx.x * 32 + threadIdx.x % 32, k = blockIdx.y, strand = threadIdx.x / 32;
+__global__ __launch_bounds__(1024) void cols_kernel(int parts, int width, const float* __restrict__ part, W* __restrict__ dw, W* __restrict__ db) {
+  __shared__ float t[64][17];
+  const int c = blockIdx.x * 16 + threadIdx.x % 16, k = blockIdx.y, strand = threadIdx.x / 16;
   W* out = k ? db : dw;
   if (!out) return;
   float a = 0.f;
   if (c < width) {
 #pragma unroll 8
-    for (int p = strand; p < parts; p += 8) a += part[((size_t)p * 2 + k) * width + c];
+    for (int p = strand; p < parts; p += 64) a += part[((size_t)p * 2 + k) * width + c];
   }
-  t[strand][threadIdx.x % 32] = a;
+  t[strand][threadIdx.x % 16] = a;
   __syncthreads();
   if (strand == 0 && c < width) {
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += t[i][threadIdx.x];
+    for (int i = 0; i < 64; ++i) s += t[i][threadIdx.x];
     out[c] = (W)s;
   }
 }
@@ -227,7 +266,8 @@ void launch(const Args& a) {
                        (T*)a.y, a.ys, a.mean, a.rstd);
 }
 
-// lanes and elements per lane by width: the fewest lanes that hold a row in at most 16 (the widest rows: 32) registers per array
+// lanes and elements per lane by width: the fewest lanes that hold a row in at most 16 registers per array.  (Rows of 1025 .. 2048 with 8 registers in 256
+// lanes rather than with 32 in one wave, which leaves one wave per SIMD: backward 32749 x 2048 bf16 88 against 112 us.)
 template <typename T, typename W, int V, bool BWD>
 void by_width(const Args& a) {
   constexpr int V4 = V == 1 ? 1 : 4;
@@ -235,9 +275,10 @@ void by_width(const Args& a) {
   else if (a.width <= 64) launch<T, W, 16, 4, V4, BWD>(a);
   else if (a.width <= 256) launch<T, W, 64, 4, V4, BWD>(a);
   else if (a.width <= 1024) launch<T, W, 64, 16, V, BWD>(a);
+  else if (a.width <= 2048) launch<T, W, 256, 8, V, BWD>(a);
   else if (a.width <= 4096) launch<T, W, 256, 16, V, BWD>(a);
   else if (a.width <= 8192) launch<T, W, 512, 16, V, BWD>(a);
-  else launch<T, W, 512, 32, V, BWD>(a);
+  else launch<T, W, 1024, 16, V, BWD>(a);
 }
 
 int groups_per_block(int width) { return width <= 32 ? 32 : width <= 64 ? 16 : width <= 1024 ? 4 : 1; }
@@ -315,11 +356,11 @@ int dpt_layer_norm_bwd(int32_t type, int32_t wtype, int64_t rows, int32_t width,
     if (rc) return rc;
   }
   if (cols) {
-    const dim3 grid((width + 31) / 32, 2);
+    const dim3 grid((width + 15) / 16, 2);
     if (wtype == DPT_F32)
-      hipLaunchKernelGGL(dptn::cols_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, parts, width, (const float*)ws, (float*)dweight, (float*)dbias);
+      hipLaunchKernelGGL(dptn::cols_kernel<float>, grid, dim3(1024), 0, (hipStream_t)stream, parts, width, (const float*)ws, (float*)dweight, (float*)dbias);
     else
-      hipLaunchKernelGGL(dptn::cols_kernel<__bf16>, grid, dim3(256), 0, (hipStream_t)stream, parts, width, (const float*)ws, (__bf16*)dweight, (__bf16*)dbias);
+      hipLaunchKernelGGL(dptn::cols_kernel<__bf16>, grid, dim3(1024), 0, (hipStream_t)stream, parts, width, (const float*)ws, (__bf16*)dweight, (__bf16*)dbias);
   }
   return (int)hipGetLastError();
 }
