@@ -46,6 +46,10 @@ template <> struct Tr<float> {
   }
 };
 
+// four neighbouring elements at any address (the memory system takes them unaligned)
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Four { T v[4]; };
+
 // 16-byte chunks per row of a tile of DP elements, and the permutation of a row's chunks in LDS that keeps both kinds of reads (32 rows at one
 // chunk; 4 rows at 4 neighbouring chunks) on different banks.  Linear over xor, and only the low 4 bits of the row count.
 template <typename T, int DP> constexpr int NC = DP * (int)sizeof(T) / 16;

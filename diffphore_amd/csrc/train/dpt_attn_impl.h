@@ -50,15 +50,26 @@ template <typename T, bool BIAS> constexpr bool FAST = sizeof(T) == 2 && !BIAS;
 // row of the wave sees only a part of the tile
 template <typename T, bool BIAS>
 __device__ __forceinline__ void finish_scores(const Dev& d, f16v& s, int key0, int h, int lim, bool part, const T* __restrict__ bias) {
+  if constexpr (BIAS) {
+    const bool unit = d.a.bias_pair == 1;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int key = key0 + 8 * (e >> 2) + 4 * h + (e & 3);
-    if constexpr (BIAS) {
-      const float x = s[e] * d.a.scale, bv = key < lim ? (float)bias[key * d.a.bias_pair] : NEG_INF;
-      s[e] = bv == NEG_INF ? NEG_INF : x + bv;
-    } else if constexpr (!FAST<T, BIAS>) {
-      s[e] *= d.a.scale;
+    for (int g = 0; g < 4; ++g) {
+      const int key = key0 + 8 * g + 4 * h;
+      float bv[4];
+      if (unit && key + 4 <= lim) {
+        const Four<T> f = *reinterpret_cast<const Four<T>*>(bias + key);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bv[i] = (float)f.v[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bv[i] = key + i < lim ? (float)bias[(key + i) * d.a.bias_pair] : NEG_INF;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[4 * g + i] = bv[i] == NEG_INF ? NEG_INF : s[4 * g + i] * d.a.scale + bv[i];
     }
+  } else if constexpr (!FAST<T, BIAS>) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] *= d.a.scale;
   }
   if constexpr (!BIAS) {
     if (part) {
@@ -339,9 +350,15 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dq_kernel(De
       if constexpr (BIAS) {
         if (dbias && rb.live) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int key = key0 + 32 * j + 8 * (e >> 2) + 4 * h + (e & 3);
-            if (key < p.nk) dbias[key] = (T)s[e];
+          for (int q = 0; q < 4; ++q) {
+            const int key = key0 + 32 * j + 8 * q + 4 * h;
+            if (key + 4 <= p.nk) {
+              *reinterpret_cast<Four<T>*>(dbias + key) = Four<T>{{(T)s[4 * q], (T)s[4 * q + 1], (T)s[4 * q + 2], (T)s[4 * q + 3]}};
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (key + i < p.nk) dbias[key + i] = (T)s[4 * q + i];
+            }
           }
         }
       }

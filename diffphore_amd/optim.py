@@ -102,13 +102,13 @@ class AdamW:
     # ---- flat buffers ---------------------------------------------------------------------------------------------------
     def views(self, flat: torch.Tensor):
         """The tensors' parts of a flat buffer, in the parameters' shapes: a list, or a dict if the parameters came as one."""
-        out = [flat[b * BLOCK:b * BLOCK + n].view(p.shape) for b, n, p in zip(self.first_block, self._numel, self.params)]
+        out = [flat[b * BLOCK:b * BLOCK + n].view(s) for b, n, s in zip(self.first_block, self._numel, self._sizes)]
         return dict(zip(self.names, out)) if self.names is not None else out
 
     def _gather(self, flat):
         v = self.views(flat)
-        for dst, p in zip(v.values() if isinstance(v, dict) else v, self.params):
-            dst.copy_(p.detach())
+        for dst, p in zip(v.values() if isinstance(v, dict) else v, self._alias):
+            dst.copy_(p)
         return flat
 
     def ema_parameters(self):
@@ -134,7 +134,17 @@ class AdamW:
         return {"step": int(self._counter[0].item()), "state_bits": self.state_bits,
                 **{n: getattr(self, n).clone() if getattr(self, n) is not None else None for n in self._STATE}}
 
+    def _refresh(self):
+        """The bf16 parameters as the roundings of their masters."""
+        v = self.views(self.master)
+        for p, m in zip(self._alias, v.values() if isinstance(v, dict) else v):
+            p.copy_(m)
+
     def load_state_dict(self, state):
+        """The state of `state_dict`; bf16 parameters become the roundings of the loaded masters (fp32 parameters are not part of the state)."""
+        t = int(state["step"])
+        if t < 0:
+            raise ValueError(f"step = {t}")
         if state["state_bits"] != self.state_bits:
             raise ValueError(f"the state has {state['state_bits']} bits, the optimiser {self.state_bits}")
         for n in self._STATE:
@@ -144,9 +154,8 @@ class AdamW:
         for n in self._STATE:
             if getattr(self, n) is not None:
                 getattr(self, n).copy_(state[n])
-        t = int(state["step"])
-        if t < 0:
-            raise ValueError(f"step = {t}")
+        if self.master is not None:
+            self._refresh()
         self._counter.copy_(torch.tensor([t, self.betas[0] ** t, self.betas[1] ** t, 0.0], dtype=torch.float64))
 
     # ---- the step -------------------------------------------------------------------------------------------------------
@@ -181,6 +190,8 @@ class AdamW:
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
         # one pass per property over the whole list: some hundreds of small tensors are the common case, and a loop over all of them costs more than the step
         some = grads if type(None) not in set(map(type, grads)) else [g for g in grads if g is not None]
+        if not all(issubclass(c, torch.Tensor) for c in set(map(type, some))):
+            raise TypeError(f"gradients are tensors or None, got {set(map(type, some))}")
         types = set(map(_DTYPE, some)) or {self.dtype}
         if len(types) > 1 or not types <= {self.dtype, torch.float32}:
             raise TypeError(f"gradients in {types}: all in {self.dtype}, or all in float32")

@@ -195,3 +195,36 @@ def test_refusals():
     with pytest.raises(ValueError):
         opt.ema_parameters()
     assert torch.equal(a, torch.ones(8, device="cuda"))
+
+
+def test_loading_bf16_state_refreshes_the_parameters():
+    params, opt, grads = _setup("bf16", 32, False)
+    opt.step(grads())
+    saved = opt.state_dict()
+    want = [p.clone() for p in params]
+    opt.step(grads())
+    opt.load_state_dict(saved)
+    assert all(torch.equal(p, w) for p, w in zip(params, want)) and opt.state_dict()["step"] == 1
+    with pytest.raises(TypeError):
+        opt.step([1.0] * len(params))
+    with pytest.raises(ValueError):
+        opt.load_state_dict({**saved, "step": -1})
+
+
+def test_parameters_pointed_elsewhere_are_not_written_through():
+    """the optimiser writes to the memory that the tensors had, which it keeps alive"""
+    p = torch.ones(300, device="cuda")
+    old = p.data
+    opt = optim.AdamW([p], lr=0.1)
+    p.data = torch.zeros(300, device="cuda")
+    opt.step([torch.ones(300, device="cuda")])
+    assert not p.any() and (old < 1).all()
+
+
+def test_small_and_absent_eps_with_moments_next_to_underflow():
+    """sqrt(v) of second moments below 2^-126 still counts when eps does not cover it"""
+    p = torch.zeros(6, device="cuda")
+    opt = optim.AdamW([p], lr=1.0, betas=(0.0, 0.5), eps=0.0, weight_decay=0.0)
+    opt.step([torch.tensor([1e-15, 1e-18, 3e-20, 1e3, 1e15, -1e-18], device="cuda")])
+    # m / sqrt(v / (1 - b2)) = 1; 9e-40 / 2 in fp32 has 18 bits left
+    assert torch.allclose(p.cpu(), torch.tensor([-1.0, -1, -1, -1, -1, 1]), rtol=1e-5)

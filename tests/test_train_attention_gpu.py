@@ -246,3 +246,53 @@ def test_refusals():
                  (do, q, k, v, out[:, :2], stats, plan), (do, q, k, v, out, stats.double(), plan)):
         with pytest.raises((TypeError, ValueError)):
             layers.attention_backward(*args)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads, kv_heads, dim", [(1, 1, 1), (40, 1, 8), (12, 2, 64), (3, 3, 2)])
+def test_one_dimension_and_many_heads_on_one_key_head(heads, kv_heads, dim, dtype):
+    check(*make([3, 40, 1], [5, 70, 33], heads, kv_heads, dim, dtype, True), causal=True)
+    check(*make([90], [200], heads, kv_heads, dim, dtype), causal=True)
+
+
+@pytest.mark.parametrize("scale", [1e-3, 1.0, 30.0])
+def test_scales(scale):
+    """from almost uniform rows to rows that one key decides; the running base follows maxima that move far"""
+    check(*make([70, 5], [300, 90], 2, 2, 32, "f32"), scale=scale)
+    q, k, v, do, b, plan = make([64], [256], 2, 1, 64, "bf16")
+    k = (k.float() * torch.linspace(0.01, 3, 256, device="cuda")[:, None, None]).bfloat16()    # scores grow along the keys
+    out, stats = layers.attention_forward(q, k, v, plan, scale=scale)
+    (o, bo), (m, bm), (l, bl) = R.attention(q, k, v, [0, 64], [0, 256], None, False, scale)
+    # exp2(fma(x, c, -m c)): the product m c is rounded once, a relative error of |m| 2^-24 (times log 2) in every term
+    extra = 2 * R.F32 * m.abs()
+    R.within(stats[0], m, bm + extra, "m")
+    R.within(stats[1], l, bl + l * extra, "l")
+    R.within(out, o, bo + 2 * extra.t()[:, :, None] * v.abs().max().double().cpu(), "out")
+
+
+def test_two_captured_graphs_with_workspaces_of_their_own():
+    q, k, v, do, b, plan = make([2, 1], [3000, 900], 8, 2, 64, "bf16")
+    inputs = [[t.clone() for t in (q, k, v)] for _ in range(2)]
+    inputs[1][0].mul_(2.0)
+    layers.attention_forward(*inputs[0], plan, causal=True)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for a in inputs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(layers.attention_forward(*a, plan, causal=True))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for i in range(3):
+        for a in inputs:
+            a[2].add_(0.5)
+        for s, g in zip(streams, graphs):                      # side by side
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                g.replay()
+        for s in streams:
+            torch.cuda.current_stream().wait_stream(s)
+        for a, (o, st) in zip(inputs, outs):
+            oe, ste = layers.attention_forward(*a, plan, causal=True)
+            torch.cuda.synchronize()
+            assert torch.equal(o, oe) and torch.equal(st, ste), i

@@ -108,7 +108,8 @@ def attention(q, k, v, q_ptr, k_ptr, bias=None, causal=False, scale=None, dout=N
             etot = (e * rel).sum(1, keepdim=True) + (nk + 4) * F32 * tot
             div = torch.where(tot == 0, 1.0, tot)
             P = e / div
-            eP = P * (rel + etot / div + 8 * F32)
+            # ... and an exponential below 2^-126, the smallest normal 32-bit number, is 0: an absolute error of up to that (over tot >= 1)
+            eP = P * (rel + etot / div + 8 * F32) + torch.where(s == -math.inf, 0.0, 2.0 ** -126)
             o = P @ V
             if dout is None:
                 out[i0:i1, h], m[h, i0:i1], l[h, i0:i1] = o, top[:, 0], tot[:, 0]
