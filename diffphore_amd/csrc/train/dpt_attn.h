@@ -26,6 +26,8 @@ struct Dev {                     // DptAttnArgs plus what every workgroup would 
   int vec;                       // rows of q, k, v, dout may be read, out and gradients written, 16 bytes at a time
   float *delta, *fac0, *fac1;    // backward, [heads, n_q] each: sum_d dout out; what turns a score into a probability (Probs)
   float *part_o, *part_ml;       // forward with splits: [splits, n_q, heads, dim] and [splits, 2, heads, n_q]
+  int splits_q, splits_k;        // backward: key ranges of a row block (dq), row ranges of a key block (dk, dv) that are summed afterwards
+  float* part_g;                 // [splits_q, n_q, heads, dim], then [splits_k, 2, n_k, kv_heads, dim]: the one is summed before the other is written
 };
 
 __device__ __forceinline__ int div_group(const Dev& d, int r) { return d.group == 1 ? r : (int)__umulhi((uint32_t)r, d.magic); }

@@ -15,34 +15,49 @@ int check(const DptAttnArgs* a) {
   const int64_t group = a->heads / a->kv_heads, rows = (int64_t)a->max_nq * group;
   // 32-bit row numbers, and their division by a multiplication; 32-bit workgroup numbers (32 rows or keys each at the least, 64 splits at the most)
   if (rows * group >= (int64_t)1 << 31 || (rows / 32 + 1) * a->B * a->kv_heads * 64 >= (int64_t)1 << 31 ||
-      ((int64_t)a->max_nk / 32 + 1) * a->B * a->kv_heads >= (int64_t)1 << 31) return DPT_E_TOOLARGE;
+      ((int64_t)a->max_nk / 32 + 1) * a->B * a->kv_heads * 64 >= (int64_t)1 << 31) return DPT_E_TOOLARGE;
   return DPT_OK;
 }
 
 // Row blocks of 32 (one wave) where the largest complex has few rows: a block of 128 would leave waves without rows; otherwise 128.
 bool small_rows(const DptAttnArgs* a) { return (int64_t)a->max_nq * (a->heads / a->kv_heads) <= 64; }
+bool small_keys(const DptAttnArgs* a) { return a->max_nk <= 64; }
 
-int splits_of(const DptAttnArgs* a) {
-  if (a->splits) return a->splits > 64 ? 64 : a->splits;
-  const int bm = small_rows(a) ? 32 : 128;
-  const int64_t rows = (int64_t)a->max_nq * (a->heads / a->kv_heads), blocks = (rows + bm - 1) / bm * a->B * a->kv_heads;
-  if (blocks == 0 || a->max_nk <= 256) return 1;
-  // enough workgroups for the chip, ranges of 128 keys at the least
-  const int64_t want = (small_rows(a) ? 4 * CUS : CUS) / blocks, most = a->max_nk / 128;
-  const int64_t s = want < most ? want : most;
+// Ranges of an axis of `length` that `blocks` workgroups walk along, each in turn: where they do not fill the chip the axis is split and the ranges' results are
+// joined afterwards.  `room`: workgroups that the chip holds at once; a range is no shorter than `least`.
+int ranges(int64_t blocks, int64_t length, int64_t room, int64_t least) {
+  if (blocks == 0) return 1;
+  const int64_t want = room / blocks, most = length / least, s = want < most ? want : most;
   return s < 2 ? 1 : s > 64 ? 64 : (int)s;
 }
 
-struct Ws { size_t delta, part_o, part_ml, total; };
-Ws layout(const DptAttnArgs* a, bool backward, int splits) {
+struct Splits { int fwd, q, k; };
+Splits splits_of(const DptAttnArgs* a) {
+  const int64_t rows = (int64_t)a->max_nq * (a->heads / a->kv_heads), bm = small_rows(a) ? 32 : 128, bk = small_keys(a) ? 32 : 128;
+  const int64_t row_blocks = (rows + bm - 1) / bm * a->B * a->kv_heads, key_blocks = (a->max_nk + bk - 1) / bk * a->B * a->kv_heads;
+  if (a->splits) {
+    const int s = a->splits > 64 ? 64 : a->splits;
+    return {s, s, s};
+  }
+  Splits s;
+  s.fwd = a->max_nk <= 256 ? 1 : ranges(row_blocks, a->max_nk, small_rows(a) ? 4 * CUS : CUS, 128);
+  // (backward: a join is another launch and 32 bits per value and range, so ranges are longer; one generation of workgroups is enough)
+  s.q = ranges(row_blocks, a->max_nk, small_rows(a) ? 4 * CUS : CUS, 256);
+  s.k = ranges(key_blocks, rows, small_keys(a) ? 4 * CUS : CUS, 256);
+  return s;
+}
+
+struct Ws { size_t delta, part_ml, total; };
+Ws layout(const DptAttnArgs* a, bool backward, const Splits& s) {
   Ws w{};
   const size_t plane = (size_t)a->heads * a->n_q * sizeof(float);
   if (backward) {
-    w.delta = up(plane);                 // one of three planes
-    w.total = 3 * w.delta;
-  } else if (splits > 1) {
-    w.part_ml = up(plane * a->dim * splits);
-    w.total = w.part_ml + up(2 * plane * splits);
+    w.delta = up(plane);                 // one of three planes, the parts of split gradients behind them
+    const size_t q = s.q > 1 ? plane * a->dim * s.q : 0, k = s.k > 1 ? (size_t)a->n_k * a->kv_heads * a->dim * sizeof(float) * 2 * s.k : 0;
+    w.total = 3 * w.delta + up(q > k ? q : k);
+  } else if (s.fwd > 1) {
+    w.part_ml = up(plane * a->dim * s.fwd);
+    w.total = w.part_ml + up(2 * plane * s.fwd);
   }
   return w;
 }
@@ -63,7 +78,7 @@ Dev dev(const DptAttnArgs* a, bool backward) {
   d.group = a->heads / a->kv_heads;
   d.magic = d.group > 1 ? (uint32_t)((((uint64_t)1 << 32) + d.group - 1) / d.group) : 0;
   d.vec = vec(a, backward);
-  d.splits = 1;
+  d.splits = d.splits_q = d.splits_k = 1;
   return d;
 }
 
@@ -98,8 +113,9 @@ int dpt_attn_fwd(const DptAttnArgs* a, void* stream) {
   if (a->B == 0 || a->n_q == 0) return DPT_OK;
   if (!a->q || !a->out || !a->stats || !a->q_ptr || !a->k_ptr || !a->pair_ptr || !a->order || (a->n_k > 0 && (!a->k || !a->v)) || dptat::strides_bad(a)) return DPT_E_BADARG;
   dptat::Dev d = dptat::dev(a, false);
-  d.splits = dptat::splits_of(a);
-  const dptat::Ws w = dptat::layout(a, false, d.splits);
+  const dptat::Splits s = dptat::splits_of(a);
+  d.splits = s.fwd;
+  const dptat::Ws w = dptat::layout(a, false, s);
   if (w.total && (!a->ws || a->ws_bytes < w.total || (uintptr_t)a->ws % 16)) return DPT_E_BADARG;
   d.part_o = (float*)a->ws;
   d.part_ml = (float*)((char*)a->ws + w.part_ml);
@@ -117,13 +133,17 @@ int dpt_attn_bwd(const DptAttnArgs* a, void* stream) {
   if (!a->q_ptr || !a->k_ptr || !a->pair_ptr || !a->order || dptat::strides_bad(a) || a->dout_row < 0 || a->dout_head < 0) return DPT_E_BADARG;
   if (a->n_q > 0 && (!a->q || !a->out || !a->stats || !a->dout || !a->dq)) return DPT_E_BADARG;
   if (a->n_k > 0 && (!a->k || !a->v || !a->dk || !a->dv)) return DPT_E_BADARG;
-  const dptat::Ws w = dptat::layout(a, true, 1);
+  const dptat::Splits s = dptat::splits_of(a);
+  const dptat::Ws w = dptat::layout(a, true, s);
   if (w.total && (!a->ws || a->ws_bytes < w.total || (uintptr_t)a->ws % 16)) return DPT_E_BADARG;
   dptat::Dev d = dptat::dev(a, true);
   d.delta = (float*)a->ws;
   d.fac0 = (float*)((char*)a->ws + w.delta);
   d.fac1 = (float*)((char*)a->ws + 2 * w.delta);
-  const bool sr = dptat::small_rows(a), sk = a->max_nk <= 64;
+  d.part_g = (float*)((char*)a->ws + 3 * w.delta);
+  d.splits_q = s.q;
+  d.splits_k = s.k;
+  const bool sr = dptat::small_rows(a), sk = dptat::small_keys(a);
   using namespace dptat;
   return (int)(a->type == DPT_F32 ? pick(a->dim, bwd_f32_32, bwd_f32_64, bwd_f32_128) : pick(a->dim, bwd_bf16_32, bwd_bf16_64, bwd_bf16_128))(d, sr, sk, (hipStream_t)stream);
 }

@@ -263,14 +263,16 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dq_kernel(De
   constexpr int NT = 64 * NW, BM = 32 * NW, J = BN / 32;
   const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
   int tile;
-  const Place p = place(d, blockIdx.x, &tile);
+  const int split = blockIdx.x % d.splits_q;
+  const Place p = place(d, blockIdx.x / d.splits_q, &tile);
   const int tiles = (p.rows + BM - 1) / BM;
   if (tile >= tiles) return;
   if (d.a.causal) tile = tiles - 1 - tile;
   const RowBlock<BM> rb(d, p, tile, lane);
   const Row row = rb.row;
   // a bias gradient is written for every pair, 0 for those behind the causal edge
-  const int ktiles = ((BIAS && d.a.dbias ? p.nk : rb.last) + BN - 1) / BN;
+  const int ktiles = ((BIAS && d.a.dbias ? p.nk : rb.last) + BN - 1) / BN, per = (ktiles + d.splits_q - 1) / d.splits_q;
+  const int t0 = split * per, t1 = min(t0 + per, ktiles);
 
   const T* kb = (const T*)d.a.k + (int64_t)p.k0 * d.a.k_row + p.hk * d.a.k_head;
   const T* vb = (const T*)d.a.v + (int64_t)p.k0 * d.a.v_row + p.hk * d.a.v_head;
@@ -278,14 +280,14 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dq_kernel(De
     stage<T, DP, BN, NT, VEC>(kt, d.a.dim, kb + (int64_t)t * BN * d.a.k_row, d.a.k_row, p.nk - t * BN);
     stage<T, DP, BN, NT, VEC>(vt, d.a.dim, vb + (int64_t)t * BN * d.a.v_row, d.a.v_row, p.nk - t * BN);
   };
-  if (ktiles) fetch(kt0, vt0, 0);
+  if (t0 < t1) fetch(kt0, vt0, t0);
   zero_pad<T, DP, BN, NT, VEC>(kt0, d.a.dim);
   zero_pad<T, DP, BN, NT, VEC>(vt0, d.a.dim);
   zero_pad<T, DP, BN, NT, VEC>(kt1, d.a.dim);
   zero_pad<T, DP, BN, NT, VEC>(vt1, d.a.dim);
 
   const int64_t at = row.token * d.a.heads + row.head, st = (int64_t)row.head * d.a.n_q + row.token, plane = (int64_t)d.a.heads * d.a.n_q;
-  const bool one = p.nk <= BN;
+  const bool one = p.nk <= BN && d.splits_q == 1;
   typename Tr<T>::frag qf[NC<T, DP> / 2], gf[NC<T, DP> / 2];
   float delta = 0.f;
   {
@@ -365,18 +367,19 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dq_kernel(De
       cols_times<DP>(kt, 32 * j, lane, (const float*)&s, dq);
     }
   };
-  for (int t = 0; t < ktiles; t += 2) {
+  for (int t = t0; t < t1; t += 2) {
     tile_barrier();
-    if (t + 1 < ktiles) fetch(kt1, vt1, t + 1);
+    if (t + 1 < t1) fetch(kt1, vt1, t + 1);
     work(kt0, vt0, t);
-    if (t + 1 >= ktiles) break;
+    if (t + 1 >= t1) break;
     tile_barrier();
-    if (t + 2 < ktiles) fetch(kt0, vt0, t + 2);
+    if (t + 2 < t1) fetch(kt0, vt0, t + 2);
     work(kt1, vt1, t + 1);
   }
   if (!rb.live) return;
-  store_col<T, DP, VEC>((T*)d.a.dq + at * d.a.dim, h, d.a.dim, dq, d.a.scale);
-  if (h == 0) {
+  if (d.splits_q == 1) store_col<T, DP, VEC>((T*)d.a.dq + at * d.a.dim, h, d.a.dim, dq, d.a.scale);
+  else store_col<float, DP, VEC>(d.part_g + (split * plane + at) * d.a.dim, h, d.a.dim, dq, d.a.scale);
+  if (h == 0 && split == 0) {
     d.delta[st] = delta;
     d.fac0[st] = f.f0;
     if (!FAST<T, BIAS>) d.fac1[st] = f.f1;
@@ -399,7 +402,8 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> && DP <= 64 ? 2 : 1)) void 
   constexpr int NT = 64 * NW, BM = 32 * NW, J = BR / 32;
   const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
   int tile;
-  const Place p = place(d, blockIdx.x, &tile);
+  const int split = blockIdx.x % d.splits_k;
+  const Place p = place(d, blockIdx.x / d.splits_k, &tile);
   if (tile * BM >= p.nk) return;
   const int key0 = tile * BM, w0 = key0 + (threadIdx.x & ~63) / 2, key = w0 + l31;
   const bool live = key < p.nk;
@@ -407,7 +411,8 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> && DP <= 64 ? 2 : 1)) void 
   // rows that see key j of the complex: from (j + n_queries - n_keys) group on (causal), all otherwise
   auto rows_from = [&](int j) __attribute__((always_inline)) { return d.a.causal ? clampi(j + p.nq - p.nk, p.nq) * d.group : 0; };
   const int rmin = rows_from(key), r_lo = __builtin_amdgcn_readfirstlane(rows_from(w0)), r_hi = __builtin_amdgcn_readfirstlane(rows_from(w0 + 31));
-  const int first = rows_from(key0) / BR, last = (p.rows + BR - 1) / BR;
+  const int begin = rows_from(key0) / BR, end = (p.rows + BR - 1) / BR, per = (end - begin + d.splits_k - 1) / d.splits_k;
+  const int first = begin + split * per, last = min(first + per, end);
 
   const int li = div_group(d, threadIdx.x / NC<T, DP>), lg = threadIdx.x / NC<T, DP> - li * d.group;
   const uint32_t q_off = (uint32_t)li * (uint32_t)d.a.q_row + (uint32_t)lg * (uint32_t)d.a.q_head, g_off = (uint32_t)li * (uint32_t)d.a.dout_row + (uint32_t)lg * (uint32_t)d.a.dout_head;
@@ -512,8 +517,27 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> && DP <= 64 ? 2 : 1)) void 
   }
   if (live) {
     const int64_t at = (token * d.a.kv_heads + p.hk) * d.a.dim;
-    store_col<T, DP, VEC>((T*)d.a.dk + at, h, d.a.dim, dk, d.a.scale);
-    store_col<T, DP, VEC>((T*)d.a.dv + at, h, d.a.dim, dv, 1.f);
+    if (d.splits_k == 1) {
+      store_col<T, DP, VEC>((T*)d.a.dk + at, h, d.a.dim, dk, d.a.scale);
+      store_col<T, DP, VEC>((T*)d.a.dv + at, h, d.a.dim, dv, 1.f);
+    } else {
+      const int64_t n = (int64_t)d.a.n_k * d.a.kv_heads * d.a.dim;
+      store_col<float, DP, VEC>(d.part_g + 2 * split * n + at, h, d.a.dim, dk, d.a.scale);
+      store_col<float, DP, VEC>(d.part_g + (2 * split + 1) * n + at, h, d.a.dim, dv, 1.f);
+    }
+  }
+}
+
+// sums the ranges' shares of a gradient, in the ranges' order; blockIdx.y: the second of two gradients that lie side by side in every range
+template <typename T>
+__global__ __launch_bounds__(256) void sum_kernel(const float* __restrict__ part, int splits, int64_t stride, int64_t n, T* __restrict__ out0, T* __restrict__ out1) {
+  T* out = blockIdx.y ? out1 : out0;
+  part += blockIdx.y * n;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    float x = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) x += part[s * stride + i];
+    out[i] = (T)x;
   }
 }
 
@@ -535,16 +559,23 @@ hipError_t run_bwd(const Dev& d0, bool small_rows, bool small_keys, hipStream_t 
   Dev d = d0;
   const int64_t rows = (int64_t)d.a.max_nq * d.group;
   d.tiles = (int)((rows + (small_rows ? 31 : 127)) / (small_rows ? 32 : 128));
-  const unsigned n = (unsigned)((int64_t)d.tiles * d.a.B * d.a.kv_heads);
+  const unsigned n = (unsigned)((int64_t)d.tiles * d.a.B * d.a.kv_heads * d.splits_q);
+  auto sum = [&](int splits, int64_t count, int many, void* a, void* b) {
+    if (splits == 1 || count == 0) return;
+    const int64_t need = (count + 255) / 256;
+    hipLaunchKernelGGL((sum_kernel<T>), dim3((unsigned)(need < 4096 ? need : 4096), many), dim3(256), 0, st, d.part_g, splits, many * count, count, (T*)a, (T*)b);
+  };
   if (n) {
     if (small_rows) hipLaunchKernelGGL((dq_kernel<T, DP, 1, BN, BIAS, VEC>), dim3(n), dim3(64), 0, st, d);
     else hipLaunchKernelGGL((dq_kernel<T, DP, 4, BN, BIAS, VEC>), dim3(n), dim3(256), 0, st, d);
+    sum(d.splits_q, (int64_t)d.a.n_q * d.a.heads * d.a.dim, 1, d.a.dq, nullptr);
   }
   d.tiles = (d.a.max_nk + (small_keys ? 31 : 127)) / (small_keys ? 32 : 128);
-  const unsigned nk = (unsigned)((int64_t)d.tiles * d.a.B * d.a.kv_heads);
+  const unsigned nk = (unsigned)((int64_t)d.tiles * d.a.B * d.a.kv_heads * d.splits_k);
   if (nk) {
     if (small_keys) hipLaunchKernelGGL((dkv_kernel<T, DP, 1, BR, BIAS, VEC>), dim3(nk), dim3(64), 0, st, d);
     else hipLaunchKernelGGL((dkv_kernel<T, DP, 4, BR, BIAS, VEC>), dim3(nk), dim3(256), 0, st, d);
+    sum(d.splits_k, (int64_t)d.a.n_k * d.a.kv_heads * d.a.dim, 2, d.a.dk, d.a.dv);
   }
   return hipGetLastError();
 }

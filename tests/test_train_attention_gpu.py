@@ -296,3 +296,37 @@ def test_two_captured_graphs_with_workspaces_of_their_own():
             oe, ste = layers.attention_forward(*a, plan, causal=True)
             torch.cuda.synchronize()
             assert torch.equal(o, oe) and torch.equal(st, ste), i
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("causal", [False, True])
+def test_backward_of_few_workgroups_is_split_and_joined(causal, dtype):
+    """one complex, one key head: key ranges of the rows' gradient and row ranges of the keys' are summed; the same bits every time"""
+    for args in (([783], [674], 2, 1, 42, dtype), ([600, 0, 70], [900, 40, 513], 2, 2, 64, dtype, True), ([1], [2000], 4, 1, 128, dtype), ([1500], [3], 1, 1, 20, dtype, True)):
+        q, k, v, do, b, plan = make(*args)
+        check(q, k, v, do, b, plan, causal=causal)
+        out, stats = layers.attention_forward(q, k, v, plan, bias=b, causal=causal)
+        one, two = (layers.attention_backward(do, q, k, v, out, stats, plan, bias=b, causal=causal) for _ in range(2))
+        assert all(x is None or torch.equal(x, y) for x, y in zip(one, two))
+
+
+def test_forced_splits_of_the_backward_pass():
+    """DptAttnArgs.splits through the C ABI: more ranges than there are tiles, empty complexes among them"""
+    import ctypes as C
+    from diffphore_amd import _trainlib
+    q, k, v, do, b, plan = make([40, 0, 3], [300, 9, 0], 4, 2, 32, "f32", True)
+    out, stats = layers.attention_forward(q, k, v, plan, bias=b)
+    ref = R.attention(q, k, v, plan.q_ptr.tolist(), plan.k_ptr.tolist(), b, dout=do)
+    L = _trainlib.lib()
+    for splits in (1, 2, 5, 64):
+        a = layers._attn_args(q, k, v, plan, b, False, 1 / math.sqrt(32))
+        a.dout_row, a.dout_head, _ = do.stride()
+        got = [torch.full_like(t, math.nan) for t in (q, k, v, b)]
+        a.splits, (a.out, a.stats, a.dout, a.dq, a.dk, a.dv, a.dbias) = splits, (t.data_ptr() for t in (out, stats, do, *got))
+        ws = torch.empty(L.dpt_attn_ws_bytes(C.byref(a), 1), dtype=torch.uint8, device="cuda")
+        a.ws, a.ws_bytes = ws.data_ptr(), ws.numel()
+        assert L.dpt_attn_bwd(C.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+        for g, r, name in zip(got, ref, ("dq", "dk", "dv", "dbias")):
+            R.within(g, *r, f"{name}, {splits} splits")
+        a.ws_bytes = 16
+        assert L.dpt_attn_bwd(C.byref(a), torch.cuda.current_stream().cuda_stream) == -1
