@@ -80,8 +80,19 @@ __global__ __launch_bounds__(64 * WAVES, 6) void step_kernel(DptAdamWArgs a, Gra
   const float b1 = (float)a.beta1, omb1 = (float)(1.0 - a.beta1), b2 = (float)a.beta2, omb2 = (float)(1.0 - a.beta2);
   const float lr1 = (float)(lr / (1.0 - p1)), ic2 = (float)(1.0 / (1.0 - p2)), eps = (float)a.eps;
   const float ema_d = (float)a.ema_decay, ema_o = (float)(1.0 - a.ema_decay), gs = a.grad_scale ? *a.grad_scale : 1.f;
-  const double k1 = (double)gs * (1.0 - a.beta1), k2 = (double)gs * (double)gs * (1.0 - a.beta2);
+  const double gsd = (double)gs, k1 = 1.0 - a.beta1, k2 = 1.0 - a.beta2;
+  const bool scaled = a.grad_scale != nullptr;
   const int lane = threadIdx.x & 63;
+  // 8 bits: what the codes stand for, as shares of the scale
+  __shared__ double m_of[BITS == 8 ? 256 : 1], v_of[BITS == 8 ? 256 : 1];
+  if constexpr (BITS == 8) {
+    static_assert(64 * WAVES == 256, "a code per lane");
+    const int c = (int)(int8_t)threadIdx.x;
+    const double r = (double)threadIdx.x / 255.0, r2 = r * r;
+    m_of[threadIdx.x] = (double)(c * abs(c)) / (127.0 * 127.0);
+    v_of[threadIdx.x] = r2 * r2;
+    __syncthreads();
+  }
   typedef const __attribute__((address_space(4))) DptAdamWBlock* Rec;      // constant memory: a wave's record is one scalar load
   auto record = [&](int i) __attribute__((always_inline)) {
     const Rec r = (Rec)(unsigned long long)(a.blocks + a.block0 + min(i, a.n_blocks - 1));
@@ -141,16 +152,19 @@ __global__ __launch_bounds__(64 * WAVES, 6) void step_kernel(DptAdamWArgs a, Gra
           x.vv[e] = x.vv[e] * b2 + g * g * omb2;
         }
       } else {
-        const double ma = (double)x.ms * (a.beta1 / (127.0 * 127.0)), va = (double)x.vs * (a.beta2 / (255.0 * 255.0 * 255.0 * 255.0));
+        const double ma = (double)x.ms, va = (double)x.vs;
         double m[4], v[4];
         float mm = 0.f, vm = 0.f, bad = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const double g = (double)x.gv[e];
-          const int c = (int)(int8_t)(x.mc >> (8 * e));
-          const unsigned q = (unsigned)(x.vc >> (8 * e)) & 255u, q2 = q * q;              // < 2^16: its square fits 32 bits
-          m[e] = fma(g, k1, ma * (double)(c * abs(c)));
-          v[e] = fma(g * g, k2, va * (double)(q2 * q2));
+          // Each operation rounded by itself, in the order of the formula.  The new scale is the largest of these rounded to 32 bits, and with betas of one
+          // decimal and bf16 gradients about one block in 130 has its largest exactly between two 32-bit numbers: a fused multiplication decides such a tie by
+          // its own last bit, and the formula evaluated in 64 bits elsewhere would get another scale.
+#pragma clang fp contract(off)
+          const double g = scaled ? (double)x.gv[e] * gsd : (double)x.gv[e];
+          const double m_old = m_of[(unsigned)(x.mc >> (8 * e)) & 255u] * ma, v_old = v_of[(unsigned)(x.vc >> (8 * e)) & 255u] * va;
+          m[e] = m_old * a.beta1 + g * k1;
+          v[e] = v_old * a.beta2 + g * g * k2;
           x.mv[e] = (float)m[e];
           x.vv[e] = (float)v[e];
           bad = fmaf(x.mv[e], 0.f, fmaf(x.vv[e], 0.f, bad));             // NaN as soon as one is not finite

@@ -228,3 +228,24 @@ def test_small_and_absent_eps_with_moments_next_to_underflow():
     opt.step([torch.tensor([1e-15, 1e-18, 3e-20, 1e3, 1e15, -1e-18], device="cuda")])
     # m / sqrt(v / (1 - b2)) = 1; 9e-40 / 2 in fp32 has 18 bits left
     assert torch.allclose(p.cpu(), torch.tensor([-1.0, -1, -1, -1, -1, 1]), rtol=1e-5)
+
+
+def test_scales_of_blocks_whose_largest_moment_is_a_tie():
+    """b1 = 0.9 and bf16 gradients: the largest new moment of a block is often exactly between two 32-bit numbers.  Its rounding is that of the formula evaluated
+    operation by operation in 64 bits - and so is every code of every block, over a million of them"""
+    g = torch.Generator().manual_seed(12)
+    n = 1 << 20
+    p = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    opt = optim.AdamW([p], lr=1e-3, betas=(0.9, 0.999), weight_decay=0.0, state_bits=8)
+    for step in range(3):
+        mc, ms, vc, vs = (t.cpu() for t in (opt.exp_avg, opt.exp_avg_scale, opt.exp_avg_sq, opt.exp_avg_sq_scale))
+        grad = (torch.randn(n, generator=g) * 1e-3).bfloat16()
+        opt.step([grad.cuda()])
+        x, c, u = grad.double(), mc.double(), vc.double() / 255.0
+        u = u * u
+        m = c * c.abs() / 127.0 ** 2 * ms.double().repeat_interleave(256) * 0.9 + x * (1.0 - 0.9)
+        v = u * u * vs.double().repeat_interleave(256) * 0.999 + x * x * (1.0 - 0.999)
+        for val, power, code, scale in ((m, 2, opt.exp_avg, opt.exp_avg_scale), (v, 4, opt.exp_avg_sq, opt.exp_avg_sq_scale)):
+            want, s = R.encode(val, power)
+            assert torch.equal(scale.cpu(), s), (step, power, "scales")
+            assert torch.equal(code.cpu(), want), (step, power, "codes")
