@@ -2,6 +2,7 @@
 //
 // Bound by HBM: every value is read once and written once.  A wave takes one 256-element block (4 elements per lane: one 16-byte load per fp32
 // array); the block's tensor comes from a table, the gradients' addresses come with the launch.  All of a step is ONE launch per 400 tensors.
+// Measured: 120 M bf16 parameters with masters and 8-bit states 550 us (3.5 TB/s), the score model's 2.2 M fp32 parameters in 228 tensors with averages 27 us.
 //
 // Step number: b1^t and b2^t live on the device (so a captured graph counts on), every workgroup reads them, and the workgroup that is the last to
 // have read them moves them on.
@@ -72,6 +73,7 @@ struct Values {
   float ms, vs;
 };
 
+// (six waves per SIMD: 540 us for the 120 M parameters against 555 with the registers that the compiler takes for four)
 template <typename P, typename G, int BITS, bool EMA>
 __global__ __launch_bounds__(64 * WAVES, 6) void step_kernel(DptAdamWArgs a, Grads grads) {
   // the step's factors, in 64 bits
@@ -246,7 +248,7 @@ __global__ __launch_bounds__(64 * WAVES, 6) void step_kernel(DptAdamWArgs a, Gra
   if (!a.last) return;
   // Every wave of this workgroup has read the counter (its products p1 and p2 are there); the last workgroup to say so moves it on and leaves the ticket
   // at 0.  No fence: nothing that this launch wrote is read by another workgroup, and the next launch sees it all.  (A device-wide fence here, which
-  // writes back the caches of its die, made 85 us of a 16 us step.)
+  // writes back the caches of its die, made the score model's step 85 us.)
   asm volatile("" ::"v"(p1), "v"(p2));
   __syncthreads();
   if (threadIdx.x == 0) {
