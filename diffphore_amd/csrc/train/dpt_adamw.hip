@@ -137,8 +137,12 @@ __global__ __launch_bounds__(64 * WAVES, 6) void step_kernel(DptAdamWArgs a, Gra
   // record and then for the values that it points to
   const int stride = gridDim.x * WAVES;
   int i = blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  Values<P, G> x = fetch(i, record(i));
-  DptAdamWBlock ahead = record(i + stride);
+  Values<P, G> x;
+  DptAdamWBlock ahead;
+  if (a.n_blocks > 0) {                                      // (a list of empty tensors has no record to read)
+    x = fetch(i, record(i));
+    ahead = record(i + stride);
+  }
   for (; i < a.n_blocks; i += stride) {
     const Values<P, G> next = fetch(i + stride, ahead);
     ahead = record(i + 2 * stride);
@@ -199,7 +203,7 @@ __global__ __launch_bounds__(64 * WAVES, 6) void step_kernel(DptAdamWArgs a, Gra
           }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            cm[e] = x.mv[e] < 0.f ? -cm[e] : cm[e];
+            cm[e] = __builtin_bit_cast(int64_t, m[e]) < 0 ? -cm[e] : cm[e];
             cv[e] = vsc > 0.f && v[e] > 0.0 ? max(cv[e], 1) : cv[e];
             mc |= (unsigned)(uint8_t)cm[e] << (8 * e);
             vc |= (unsigned)cv[e] << (8 * e);

@@ -249,3 +249,16 @@ def test_scales_of_blocks_whose_largest_moment_is_a_tie():
             want, s = R.encode(val, power)
             assert torch.equal(scale.cpu(), s), (step, power, "scales")
             assert torch.equal(code.cpu(), want), (step, power, "codes")
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_lists_of_empty_tensors(bits):
+    """nothing but empty tensors, and a launch of the list whose tensors are all empty: the step counts, nothing is read"""
+    empty = optim.AdamW([torch.empty(0, 3, device="cuda")], state_bits=bits, ema_decay=0.9)
+    empty.step([torch.empty(0, 3, device="cuda")])
+    assert empty.state_dict()["step"] == 1
+    params = [torch.ones(7, device="cuda")] + [torch.empty(0, device="cuda") for _ in range(900)]
+    opt = optim.AdamW(params, lr=0.5, weight_decay=0.0, state_bits=bits)
+    opt.step([torch.ones_like(p) for p in params])
+    opt.step([torch.ones_like(p) for p in params])
+    assert opt.state_dict()["step"] == 2 and torch.allclose(params[0], torch.zeros(7, device="cuda"), atol=0.02)
