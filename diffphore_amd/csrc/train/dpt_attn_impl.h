@@ -487,18 +487,19 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> && DP <= 64 ? 2 : 1)) void 
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] *= d.a.scale;
       }
+      unsigned seen = 0xffffu;                               // a bit per entry
       if (part || BIAS) {
+        seen = 0;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int rr = 32 * j + 8 * (e >> 2) + 4 * h + (e & 3), r = r0 + rr;
-          bool seen = live && r >= rmin && r < p.rows;
+          bool in = live && r >= rmin && r < p.rows;
           if constexpr (BIAS) {
-            const float bv = seen ? (float)((const T*)d.a.bias)[rt.bias[rr] + key * d.a.bias_pair] : NEG_INF;
+            const float bv = in ? (float)((const T*)d.a.bias)[rt.bias[rr] + key * d.a.bias_pair] : NEG_INF;
             s[e] += bv;
-            seen = bv != NEG_INF;
+            in = bv != NEG_INF;
           }
-          s[e] = seen ? s[e] : NEG_INF;
-          g[e] = seen ? g[e] : 0.f;
+          seen |= (unsigned)in << e;
         }
       }
 #pragma unroll
@@ -506,6 +507,13 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> && DP <= 64 ? 2 : 1)) void 
         const int rr = 32 * j + 8 * (e >> 2) + 4 * h + (e & 3);
         s[e] = Probs<T, BIAS>::p(s[e], c, rt.f0[rr], FAST<T, BIAS> ? 0.f : rt.f1[rr]);
         g[e] = s[e] * (g[e] - rt.delta[rr]);
+      }
+      if (part || BIAS) {                                    // chosen, not multiplied: scores, statistics and do.v of what is taken out may be anything
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          s[e] = seen >> e & 1 ? s[e] : 0.f;
+          g[e] = seen >> e & 1 ? g[e] : 0.f;
+        }
       }
       cols_times<DP>(rt.g, 32 * j, lane, (const float*)&s, dv);
       cols_times<DP>(rt.q, 32 * j, lane, (const float*)&g, dk);

@@ -330,3 +330,20 @@ def test_forced_splits_of_the_backward_pass():
             R.within(g, *r, f"{name}, {splits} splits")
         a.ws_bytes = 16
         assert L.dpt_attn_bwd(C.byref(a), torch.cuda.current_stream().cuda_stream) == -1
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_row_that_is_nan_leaves_the_values_that_it_does_not_see(dtype, bias):
+    """causal: query 3 is NaN, so are its statistics; dv of the keys behind it, and dbias of the other rows, are those of the rows that see them"""
+    q, k, v, do, b, plan = make([40], [40], 1, 1, 32, dtype, bias)
+    out, stats = layers.attention_forward(q, k, v, plan, bias=b, causal=True)
+    _, _, dv, db = layers.attention_backward(do, q, k, v, out, stats, plan, bias=b, causal=True)
+    q[3] = math.nan
+    out, stats = layers.attention_forward(q, k, v, plan, bias=b, causal=True)
+    assert torch.isnan(out[3]).all() and torch.isfinite(out[4:]).all()
+    _, _, dv2, db2 = layers.attention_backward(do, q, k, v, out, stats, plan, bias=b, causal=True)
+    assert torch.equal(dv2[4:], dv[4:]) and torch.isnan(dv2[:4]).all()
+    if bias:
+        rest = [i for i in range(40) if i != 3]
+        assert torch.equal(db2.view(1, 40, 40)[:, rest], db.view(1, 40, 40)[:, rest])
