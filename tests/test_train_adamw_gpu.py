@@ -262,3 +262,12 @@ def test_lists_of_empty_tensors(bits):
     opt.step([torch.ones_like(p) for p in params])
     opt.step([torch.ones_like(p) for p in params])
     assert opt.state_dict()["step"] == 2 and torch.allclose(params[0], torch.zeros(7, device="cuda"), atol=0.02)
+
+
+def test_a_transposed_gradient_is_refused():
+    p = [torch.zeros(4, 6, device="cuda"), torch.zeros(5, device="cuda")]
+    opt = optim.AdamW(p)
+    for bad in ([torch.ones(6, 4, device="cuda"), torch.ones(5, device="cuda")], [torch.ones(6, 4, device="cuda"), None], [torch.ones(4, 6, device="cuda"), torch.ones(4, device="cuda")]):
+        with pytest.raises(ValueError):
+            opt.step(bad)
+    assert not p[0].any() and not p[1].any() and opt.state_dict()["step"] == 0
