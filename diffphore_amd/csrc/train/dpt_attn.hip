@@ -43,7 +43,12 @@ int ranges(int64_t blocks, int64_t length, int64_t room, int64_t least) {
 struct Splits { int fwd, q, k; };
 Splits splits_of(const DptAttnArgs* a) {
   const int64_t rows = (int64_t)a->max_nq * (a->heads / a->kv_heads), bm = small_rows(a) ? 32 : 128, bk = small_keys(a) ? 32 : 128;
-  const int64_t row_blocks = (rows + bm - 1) / bm * a->B * a->kv_heads, key_blocks = (a->max_nk + bk - 1) / bk * a->B * a->kv_heads;
+  // workgroups that have work: by the largest complex, or by the total with half a block lost per complex, whichever is less (ragged batches)
+  auto blocks = [&](int64_t largest, int64_t total, int64_t block) {
+    const int64_t x = (largest + block - 1) / block * a->B, y = (total + a->B * (block / 2) + block - 1) / block;
+    return (x < y ? x : y) * a->kv_heads;
+  };
+  const int64_t row_blocks = blocks(rows, (int64_t)a->n_q * (a->heads / a->kv_heads), bm), key_blocks = blocks(a->max_nk, a->n_k, bk);
   if (a->splits) {
     const int s = a->splits > 64 ? 64 : a->splits;
     return {s, s, s};
