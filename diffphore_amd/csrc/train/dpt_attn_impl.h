@@ -392,7 +392,7 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dq_kernel(De
 // ---- backward: gradients of the keys and values ---------------------------------------------------------------------------------------------------
 // NW waves x 32 keys; the rows of all heads of the group in tiles of BR, the next one on its way.  Rows down, keys across: the probability and ds tiles
 // are second operands as they stand, dv[d, key] += do[row, d] p[row, key], dk[d, key] += q[row, d] ds[row, key].
-// Measured as above: 410 us (four products: 670 TFLOP/s; at a head dimension of 128 both sums and the wave's keys and values are 230 registers, so one wave per
+// Measured as above: 402 us (four products: 684 TFLOP/s; at a head dimension of 128 both sums and the wave's keys and values are 230 registers, so one wave per
 // SIMD) and 34 us.
 template <typename T, int DP, int NW, int BR, bool BIAS>
 struct RowTile {
