@@ -347,3 +347,30 @@ def test_a_row_that_is_nan_leaves_the_values_that_it_does_not_see(dtype, bias):
     if bias:
         rest = [i for i in range(40) if i != 3]
         assert torch.equal(db2.view(1, 40, 40)[:, rest], db.view(1, 40, 40)[:, rest])
+
+
+def test_offsets_beyond_32_bits():
+    """keys and values of more than 2^31 elements: a small complex behind a very long one, and the long one's last keys"""
+    n, tail, H, D = 1_060_000, 70, 16, 128
+    assert n * H * D > 1 << 31
+    g = torch.Generator().manual_seed(2)
+    k, v = (torch.zeros(n + tail, H, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    k[-tail - 1:], v[-tail - 1:] = (torch.randn(tail + 1, H, D, generator=g).bfloat16().cuda() for _ in range(2))      # the long one's last key too
+    q, do = (torch.randn(4, H, D, generator=g).bfloat16().cuda() for _ in range(2))
+    plan = layers.PairPlan([0, 1, 4], [0, n, n + tail])
+    out, stats = layers.attention_forward(q, k, v, plan)
+    (o, bo), _, _ = R.attention(q[1:], k[n:], v[n:], [0, 3], [0, tail])
+    R.within(out[1:], o, bo, "out")
+    # the long complex: n - 1 scores of 0 with values 0, and one of s.  A sum of n terms in 32 bits is good to n 2^-24 (6 %), p and the output to half a step each
+    s = (q[0].double() * k[n - 1].double()).sum(-1) / D ** 0.5
+    top, wide = s.clamp(min=0), n * R.F32 + 3 * R.U[torch.bfloat16]
+    total = torch.exp(s - top) + (n - 1) * torch.exp(-top)
+    p = torch.exp(s - top) / total
+    R.within(stats[1, :, 0], total, n * R.F32 * total, "l")
+    want = p[:, None] * v[n - 1].double()
+    R.within(out[0], want, wide * want.abs(), "out of the long complex")
+    dq, dk, dv, _ = layers.attention_backward(do, q, k, v, out, stats, plan)
+    for got, ref, name in zip((dq[1:], dk[n:], dv[n:]), R.attention(q[1:], k[n:], v[n:], [0, 3], [0, tail], dout=do[1:]), ("dq", "dk", "dv")):
+        R.within(got, *ref, name)
+    want = p[:, None] * do[0].double()
+    R.within(dv[n - 1], want, wide * want.abs(), "dv of the last key")
