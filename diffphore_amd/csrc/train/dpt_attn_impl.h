@@ -1,4 +1,4 @@
-// dpt_attn_impl.h - the attention kernels, instantiated per element type (dpt_attn_f32.hip, dpt_attn_bf16.hip).
+// dpt_attn_impl.h - the attention kernels, instantiated per element type and padded head dimension (dpt_attn_<type>_<dim>.hip).
 #pragma once
 #include "dpt_attn.h"
 
