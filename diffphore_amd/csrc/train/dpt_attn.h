@@ -23,6 +23,7 @@ struct Dev {                     // DptAttnArgs plus what every workgroup would 
   int group, splits;             // query heads per key head; key ranges
   uint32_t magic;                // r / group = mulhi(r, magic) for group > 1
   int tiles;                     // row (backward: key) blocks of the largest complex
+  int first;                     // this launch's first workgroup (in_parts)
   int vec;                       // rows of q, k, v, dout may be read, out and gradients written, 16 bytes at a time
   float *delta, *fac0, *fac1;    // backward, [heads, n_q] each: sum_d dout out; what turns a score into a probability (Probs)
   float *part_o, *part_ml;       // forward with splits: [splits, n_q, heads, dim] and [splits, 2, heads, n_q]
@@ -209,6 +210,19 @@ __device__ __forceinline__ void zero_pad(T* tile, int dim) {
     for (int e = 0; e < CH; ++e) z[e] = (T)0.f;
     if (c * CH >= dim) *reinterpret_cast<typename Tr<T>::frag*>(tile + i * CH) = z;
   }
+}
+
+// A launch's gridDim.x * blockDim.x has to stay below 2^32, and check() allows up to 2^31 workgroups of 256 lanes: more than MOST go in several launches, each
+// with the number of its first workgroup.  Ends at the first launch that fails.
+template <typename F>
+hipError_t in_parts(Dev& d, int64_t n, F launch) {
+  constexpr int64_t MOST = 1 << 23;
+  for (int64_t at = 0; at < n; at += MOST) {
+    d.first = (int)at;
+    launch((unsigned)(n - at < MOST ? n - at : MOST));
+    if (const hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
 }
 
 // dpt_attn_<type>_<padded head dimension>.hip

@@ -13,7 +13,8 @@ int check(const DptAttnArgs* a) {
   if (a->n_q < 0 || a->n_k < 0 || a->max_nq < 0 || a->max_nk < 0 || a->max_nq > a->n_q || a->max_nk > a->n_k || a->n_pairs < 0 || a->splits < 0) return DPT_E_BADARG;
   if (a->dim > 128) return DPT_E_TOOLARGE;
   const int64_t group = a->heads / a->kv_heads, rows = (int64_t)a->max_nq * group;
-  // 32-bit row numbers, and their division by a multiplication; 32-bit workgroup numbers (32 rows or keys each at the least; ranges() splits few workgroups only)
+  // 32-bit row numbers, and their division by a multiplication; 32-bit workgroup numbers, over all parts of a launch (32 rows or keys each at the least; ranges()
+  // splits few workgroups only)
   const int64_t most = ((int64_t)1 << 31) / (a->splits ? 64 : 1);
   if (rows * group >= (int64_t)1 << 31 || (rows / 32 + 1) * a->B * a->kv_heads >= most ||
       ((int64_t)a->max_nk / 32 + 1) * a->B * a->kv_heads >= most) return DPT_E_TOOLARGE;

@@ -116,7 +116,7 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void fwd_kernel(D
   constexpr int NT = 64 * NW, BM = 32 * NW, J = BN / 32;
   constexpr float FAR = 8.f;
   const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
-  int id = blockIdx.x, tile;
+  int id = d.first + blockIdx.x, tile;
   const int split = id % d.splits;
   const Place p = place(d, id / d.splits, &tile);
   const int tiles = (p.rows + BM - 1) / BM;
@@ -211,10 +211,10 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void fwd_kernel(D
   }
 }
 
-// joins the key ranges of a row: one wave per (row, head), in the ranges' order
+// joins the key ranges of a row: one wave per (row, head), in the ranges' order; d.first as above
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(Dev d) {
-  const int64_t plane = (int64_t)d.a.heads * d.a.n_q, at = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  const int64_t plane = (int64_t)d.a.heads * d.a.n_q, at = ((int64_t)d.first + blockIdx.x) * 4 + threadIdx.x / 64;
   if (at >= plane) return;
   const int lane = threadIdx.x & 63, head = (int)(at % d.a.heads);
   const int64_t st = (int64_t)head * d.a.n_q + at / d.a.heads;
@@ -265,9 +265,9 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dq_kernel(De
   __shared__ __attribute__((aligned(16))) T kt0[BN * DP], vt0[BN * DP], kt1[BN * DP], vt1[BN * DP];
   constexpr int NT = 64 * NW, BM = 32 * NW, J = BN / 32;
   const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
-  int tile;
-  const int split = blockIdx.x % d.splits_q;
-  const Place p = place(d, blockIdx.x / d.splits_q, &tile);
+  int id = d.first + blockIdx.x, tile;
+  const int split = id % d.splits_q;
+  const Place p = place(d, id / d.splits_q, &tile);
   const int tiles = (p.rows + BM - 1) / BM;
   if (tile >= tiles) return;
   if (d.a.causal) tile = tiles - 1 - tile;
@@ -406,9 +406,9 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> && DP <= 64 ? 2 : 1)) void 
   __shared__ RowTile<T, DP, NW, BR, BIAS> rt0, rt1;
   constexpr int NT = 64 * NW, BM = 32 * NW, J = BR / 32;
   const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5;
-  int tile;
-  const int split = blockIdx.x % d.splits_k;
-  const Place p = place(d, blockIdx.x / d.splits_k, &tile);
+  int id = d.first + blockIdx.x, tile;
+  const int split = id % d.splits_k;
+  const Place p = place(d, id / d.splits_k, &tile);
   if (tile * BM >= p.nk) return;
   const int key0 = tile * BM, w0 = key0 + (threadIdx.x & ~63) / 2, key = w0 + l31;
   const bool live = key < p.nk;
@@ -555,15 +555,17 @@ __global__ __launch_bounds__(256) void sum_kernel(const float* __restrict__ part
 }
 
 template <typename T, int DP, bool BIAS, bool VEC>
-hipError_t run_fwd(const Dev& d, bool small, hipStream_t st) {
+hipError_t run_fwd(const Dev& d0, bool small, hipStream_t st) {
   constexpr int BN = sizeof(T) == 2 ? 64 : 32;
-  const unsigned n = (unsigned)((int64_t)d.tiles * d.a.B * d.a.kv_heads * d.splits);
-  if (n) {
-    if (small) hipLaunchKernelGGL((fwd_kernel<T, DP, 1, BN, BIAS, VEC>), dim3(n), dim3(64), 0, st, d);
-    else hipLaunchKernelGGL((fwd_kernel<T, DP, 4, BN, BIAS, VEC>), dim3(n), dim3(256), 0, st, d);
-    if (d.splits > 1) hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(((int64_t)d.a.heads * d.a.n_q + 3) / 4)), dim3(256), 0, st, d);
-  }
-  return hipGetLastError();
+  Dev d = d0;
+  const int64_t n = (int64_t)d.tiles * d.a.B * d.a.kv_heads * d.splits;
+  hipError_t rc = in_parts(d, n, [&](unsigned part) {
+    if (small) hipLaunchKernelGGL((fwd_kernel<T, DP, 1, BN, BIAS, VEC>), dim3(part), dim3(64), 0, st, d);
+    else hipLaunchKernelGGL((fwd_kernel<T, DP, 4, BN, BIAS, VEC>), dim3(part), dim3(256), 0, st, d);
+  });
+  if (rc == hipSuccess && n && d.splits > 1)
+    rc = in_parts(d, ((int64_t)d.a.heads * d.a.n_q + 3) / 4, [&](unsigned part) { hipLaunchKernelGGL((join_kernel<T>), dim3(part), dim3(256), 0, st, d); });
+  return rc;
 }
 
 template <typename T, int DP, bool BIAS, bool VEC>
@@ -572,25 +574,25 @@ hipError_t run_bwd(const Dev& d0, bool small_rows, bool small_keys, hipStream_t 
   Dev d = d0;
   const int64_t rows = (int64_t)d.a.max_nq * d.group;
   d.tiles = (int)((rows + (small_rows ? 31 : 127)) / (small_rows ? 32 : 128));
-  const unsigned n = (unsigned)((int64_t)d.tiles * d.a.B * d.a.kv_heads * d.splits_q);
   auto sum = [&](int splits, int64_t count, int many, void* a, void* b) {
-    if (splits == 1 || count == 0) return;
+    if (splits == 1 || count == 0) return hipSuccess;
     const int64_t need = (count + 255) / 256;
     hipLaunchKernelGGL((sum_kernel<T>), dim3((unsigned)(need < 4096 ? need : 4096), many), dim3(256), 0, st, d.part_g, splits, many * count, count, (T*)a, (T*)b);
+    return hipGetLastError();
   };
-  if (n) {
-    if (small_rows) hipLaunchKernelGGL((dq_kernel<T, DP, 1, BN, BIAS, VEC>), dim3(n), dim3(64), 0, st, d);
-    else hipLaunchKernelGGL((dq_kernel<T, DP, 4, BN, BIAS, VEC>), dim3(n), dim3(256), 0, st, d);
-    sum(d.splits_q, (int64_t)d.a.n_q * d.a.heads * d.a.dim, 1, d.a.dq, nullptr);
-  }
+  // (the second kernel reads what the first one wrote: it is not started if a launch of the first failed)
+  hipError_t rc = in_parts(d, (int64_t)d.tiles * d.a.B * d.a.kv_heads * d.splits_q, [&](unsigned part) {
+    if (small_rows) hipLaunchKernelGGL((dq_kernel<T, DP, 1, BN, BIAS, VEC>), dim3(part), dim3(64), 0, st, d);
+    else hipLaunchKernelGGL((dq_kernel<T, DP, 4, BN, BIAS, VEC>), dim3(part), dim3(256), 0, st, d);
+  });
+  if (rc == hipSuccess) rc = sum(d.splits_q, (int64_t)d.a.n_q * d.a.heads * d.a.dim, 1, d.a.dq, nullptr);
+  if (rc != hipSuccess) return rc;
   d.tiles = (d.a.max_nk + (small_keys ? 31 : 127)) / (small_keys ? 32 : 128);
-  const unsigned nk = (unsigned)((int64_t)d.tiles * d.a.B * d.a.kv_heads * d.splits_k);
-  if (nk) {
-    if (small_keys) hipLaunchKernelGGL((dkv_kernel<T, DP, 1, BR, BIAS, VEC>), dim3(nk), dim3(64), 0, st, d);
-    else hipLaunchKernelGGL((dkv_kernel<T, DP, 4, BR, BIAS, VEC>), dim3(nk), dim3(256), 0, st, d);
-    sum(d.splits_k, (int64_t)d.a.n_k * d.a.kv_heads * d.a.dim, 2, d.a.dk, d.a.dv);
-  }
-  return hipGetLastError();
+  rc = in_parts(d, (int64_t)d.tiles * d.a.B * d.a.kv_heads * d.splits_k, [&](unsigned part) {
+    if (small_keys) hipLaunchKernelGGL((dkv_kernel<T, DP, 1, BR, BIAS, VEC>), dim3(part), dim3(64), 0, st, d);
+    else hipLaunchKernelGGL((dkv_kernel<T, DP, 4, BR, BIAS, VEC>), dim3(part), dim3(256), 0, st, d);
+  });
+  return rc == hipSuccess ? sum(d.splits_k, (int64_t)d.a.n_k * d.a.kv_heads * d.a.dim, 2, d.a.dk, d.a.dv) : rc;
 }
 
 template <typename T, int DP>

@@ -374,3 +374,26 @@ def test_offsets_beyond_32_bits():
         R.within(got, *ref, name)
     want = p[:, None] * do[0].double()
     R.within(dv[n - 1], want, wide * want.abs(), "dv of the last key")
+
+
+@pytest.mark.parametrize("long_keys", [False, True])
+def test_more_workgroups_than_one_launch_takes(long_keys):
+    """one long complex among a thousand short ones: the blocks of the largest complex times the complexes are more than 2^24 workgroups of 256 lanes, whose
+    lanes do not fit the 32 bits of one launch.  A short complex has one query and one key: out = v, dv = dout, dq = dk = 0"""
+    short, long, H, D = 1030, 32768, 64, 4
+    assert (long // 128) * (short + 1) * H > 1 << 24
+    nq, nk = [1] * short + [3 if long_keys else long], [1] * short + [long if long_keys else 3]
+    q, k, v, do, _, plan = make(nq, nk, H, H, D, "f32")
+    out, stats = layers.attention_forward(q, k, v, plan)
+    dq, dk, dv, _ = layers.attention_backward(do, q, k, v, out, stats, plan)
+    assert torch.equal(out[:short], v[:short]) and torch.equal(dv[:short], do[:short]) and not dq[:short].any() and not dk[:short].any()
+    assert torch.equal(stats[1, :, :short], torch.ones_like(stats[1, :, :short]))
+    for h in (0, H - 1):
+        args = [t[short:, h:h + 1] for t in (q, k, v)]
+        (o, bo), (m, bm), (l, bl) = R.attention(*args, [0, nq[-1]], [0, nk[-1]])
+        R.within(out[short:, h:h + 1], o, bo, "out")
+        R.within(stats[0, h:h + 1, short:], m, bm, "m")
+        R.within(stats[1, h:h + 1, short:], l, bl, "l")
+        refs = R.attention(*args, [0, nq[-1]], [0, nk[-1]], dout=do[short:, h:h + 1])
+        for got, ref, name in zip((dq, dk, dv), refs, ("dq", "dk", "dv")):
+            R.within(got[short:, h:h + 1], *ref, name)
