@@ -5,19 +5,21 @@ namespace dptat {
 
 constexpr int CUS = 256;
 constexpr size_t ALIGN = 256;
+constexpr int32_t MOST_ROWS = DPT_ATTN_MAX_ROWS;
 size_t up(size_t n) { return (n + ALIGN - 1) / ALIGN * ALIGN; }
 
 int check(const DptAttnArgs* a) {
   if (!a || (a->type != DPT_F32 && a->type != DPT_BF16)) return DPT_E_BADARG;
   if (a->B < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->dim < 1 || !(a->scale > 0.f) || a->scale > 3.4e38f) return DPT_E_BADARG;
   if (a->n_q < 0 || a->n_k < 0 || a->max_nq < 0 || a->max_nk < 0 || a->max_nq > a->n_q || a->max_nk > a->n_k || a->n_pairs < 0 || a->splits < 0) return DPT_E_BADARG;
-  if (a->dim > 128) return DPT_E_TOOLARGE;
+  if (a->dim > 128 || a->n_q > MOST_ROWS || a->n_k > MOST_ROWS) return DPT_E_TOOLARGE;   // the last block's row numbers, past the end, still fit
   const int64_t group = a->heads / a->kv_heads, rows = (int64_t)a->max_nq * group;
   // 32-bit row numbers, and their division by a multiplication; 32-bit workgroup numbers, over all parts of a launch (32 rows or keys each at the least; ranges()
   // splits few workgroups only)
   const int64_t most = ((int64_t)1 << 31) / (a->splits ? 64 : 1);
-  if (rows * group >= (int64_t)1 << 31 || (rows / 32 + 1) * a->B * a->kv_heads >= most ||
-      ((int64_t)a->max_nk / 32 + 1) * a->B * a->kv_heads >= most) return DPT_E_TOOLARGE;
+  if (rows > MOST_ROWS || rows * group >= (int64_t)1 << 31) return DPT_E_TOOLARGE;
+  const int64_t lists = (int64_t)a->B * a->kv_heads, longest = (rows > a->max_nk ? rows : a->max_nk) / 32 + 1;
+  if (lists >= most || longest * lists >= most) return DPT_E_TOOLARGE;
   return DPT_OK;
 }
 

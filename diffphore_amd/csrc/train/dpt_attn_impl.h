@@ -29,7 +29,7 @@ __device__ __forceinline__ Place place(const Dev& d, int id, int* tile) {
 
 __device__ __forceinline__ int clampi(int x, int hi) { return x < 0 ? 0 : x < hi ? x : hi; }
 // keys that query i of the complex sees
-__device__ __forceinline__ int keys_seen(const Dev& d, const Place& p, int i) { return d.a.causal ? clampi(i + 1 + p.nk - p.nq, p.nk) : p.nk; }
+__device__ __forceinline__ int keys_seen(const Dev& d, const Place& p, int i) { return d.a.causal ? clampi(i + 1 - p.nq + p.nk, p.nk) : p.nk; }
 
 // a lane's row: its query and head, and where it lies
 struct Row { int i, head; int64_t token; };
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> && DP <= 64 ? 2 : 1)) void 
   const bool live = key < p.nk;
   const int64_t token = p.k0 + (live ? key : p.nk - 1);
   // rows that see key j of the complex: from (j + n_queries - n_keys) group on (causal), all otherwise
-  auto rows_from = [&](int j) __attribute__((always_inline)) { return d.a.causal ? clampi(j + p.nq - p.nk, p.nq) * d.group : 0; };
+  auto rows_from = [&](int j) __attribute__((always_inline)) { return d.a.causal ? clampi(j - p.nk + p.nq, p.nq) * d.group : 0; };
   const int rmin = rows_from(key), r_lo = __builtin_amdgcn_readfirstlane(rows_from(w0)), r_hi = __builtin_amdgcn_readfirstlane(rows_from(w0 + 31));
   const int begin = rows_from(key0) / BR, end = (p.rows + BR - 1) / BR, per = (end - begin + d.splits_k - 1) / d.splits_k;
   const int first = begin + split * per, last = min(first + per, end);

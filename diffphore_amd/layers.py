@@ -19,6 +19,7 @@ from . import _trainlib
 from ._trainlib import TYPES, DptAttnArgs, call, need_gpu
 
 _LN_MAX_WIDTH = 16384
+_MAX_ROWS = 2 ** 31 - 1025                              # DPT_ATTN_MAX_ROWS
 
 
 # ----------------------------------------------------------------------------------------------------------------------
@@ -146,8 +147,8 @@ def _offsets(p, name) -> np.ndarray:
     a = a.astype(np.int64)
     if a[0] != 0 or (np.diff(a) < 0).any():
         raise ValueError(f"{name}: offsets start at 0 and do not fall")
-    if a[-1] >= 1 << 31:
-        raise ValueError(f"{name}: {a[-1]} rows do not fit 31 bits")
+    if a[-1] > _MAX_ROWS:
+        raise ValueError(f"{name}: {a[-1]} rows, at most {_MAX_ROWS} are supported")
     return a
 
 

@@ -54,6 +54,8 @@ int dpt_layer_norm_bwd(int32_t type, int32_t wtype, int64_t rows, int32_t width,
  * causal: key j of a complex is seen by query i iff j <= i + n_keys - n_queries.  A bias of -inf takes the pair out.  A row that sees nothing:
  * out = 0, m = -inf, l = 0, gradients 0.  As in every product of probabilities and values, a NaN or inf in v of a pair that is taken out still
  * reaches the rows of its tile (0 x NaN), and in the backward pass one in q, k or dout. */
+#define DPT_ATTN_MAX_ROWS (0x7fffffff - 1024) /* most rows of q (max_nq times the heads that share a key head, too) and of k */
+
 typedef struct DptAttnArgs {
   int32_t type;                    /* DptType of q, k, v, bias, out, dout and the gradients */
   int32_t B, heads, kv_heads, dim; /* dim 1 .. 128 */

@@ -148,3 +148,17 @@ def test_codes_are_nearest_and_keep_small_second_moments(power):
     small = (root(x) * top < 0.5) & (root(x) > 0) if power == 4 else torch.zeros_like(off, dtype=torch.bool)
     assert off[~small].max() <= 0.5 + 1e-5 and torch.equal(y == 0, x == 0) if power == 4 else off.max() <= 0.5 + 1e-5
     assert np.isfinite(y.numpy()).all() and code[256:512].abs().max() == 0 if power == 2 else True
+
+
+@pytest.mark.parametrize("kw", [dict(n_k=2 ** 31 - 1, max_nk=2 ** 31 - 1), dict(n_k=2 ** 31 - 1024, max_nk=8), dict(n_q=2 ** 31 - 1024, max_nq=8),
+                                dict(n_q=2 ** 31 - 1025, max_nq=2 ** 31 - 1025), dict(heads=2 ** 31 - 1, kv_heads=1, n_q=2 ** 30, max_nq=2 ** 30),
+                                dict(B=2 ** 31 - 1, heads=2 ** 31 - 1, kv_heads=2 ** 31 - 1, n_k=2 ** 30, max_nk=2 ** 30)])
+def test_lengths_and_counts_whose_arithmetic_would_wrap_are_too_large(kw):
+    """row numbers of a last block that pass 2^31, and products of sizes that pass 2^63: refused on the host (the pointers are NULL, so -1 follows otherwise)"""
+    L = _trainlib.lib()
+    a = _attn_args(**kw)
+    assert L.dpt_attn_fwd(C.byref(a), None) == -3 and L.dpt_attn_bwd(C.byref(a), None) == -3 and L.dpt_attn_ws_bytes(C.byref(a), 1) == 0
+    a = _attn_args(heads=1, kv_heads=1, n_k=2 ** 31 - 1025, max_nk=2 ** 31 - 1025)
+    assert L.dpt_attn_fwd(C.byref(a), None) == -1
+    with pytest.raises(ValueError, match="rows"):
+        layers.PairPlan([0, 1], [0, 2 ** 31 - 1024])
