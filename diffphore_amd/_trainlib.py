@@ -82,6 +82,23 @@ def call(what: str, fn, index: int, *args):
         check(rc, what)
 
 
+class Streams:
+    """Memory that an object owns and that its launches read or write on whatever stream is current: the allocator learns of every stream but the one that
+    the memory was allocated on, so that dropping the object while such a stream still works does not hand the memory out again."""
+
+    def __init__(self, device: torch.device, tensors):
+        self._index, self._tensors = device.index, [t for t in tensors if t is not None]
+        self._known = {_raw_stream(self._index)}
+
+    def use(self):
+        raw = _raw_stream(self._index)
+        if raw not in self._known:
+            stream = torch.cuda.current_stream(self._index)
+            for t in self._tensors:
+                t.record_stream(stream)
+            self._known.add(raw)
+
+
 def need_gpu(t: torch.Tensor, name: str):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: a tensor is wanted, got {type(t).__name__}")

@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _trainlib
-from ._trainlib import TYPES, DptAttnArgs, call, need_gpu
+from ._trainlib import TYPES, DptAttnArgs, Streams, call, need_gpu
 
 _LN_MAX_WIDTH = 16384
 _MAX_ROWS = 2 ** 31 - 1025                              # DPT_ATTN_MAX_ROWS
@@ -176,6 +176,7 @@ class PairPlan:
         self._dev = torch.from_numpy(host).to(self.device)
         base, n = self._dev.data_ptr(), self.B + 1
         self._ptrs = (base + 8 * n, base + 12 * n, base, base + 16 * n)         # q_ptr, k_ptr, pair_ptr, order
+        self._streams = Streams(self.device, [self._dev])
 
     @classmethod
     def from_batch(cls, batch, queries: str = "ligand", keys: str = "phore") -> "PairPlan":
@@ -223,6 +224,7 @@ def _attn_args(q, k, v, plan, bias, causal, scale) -> DptAttnArgs:
     a.q_row, a.q_head, _ = q.stride()
     a.k_row, a.k_head, _ = k.stride()
     a.v_row, a.v_head, _ = v.stride()
+    plan._streams.use()
     a.q_ptr, a.k_ptr, a.pair_ptr, a.order = plan._ptrs
     a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
     if bias is not None:

@@ -15,7 +15,7 @@ import numpy as np
 import torch
 
 from . import _trainlib
-from ._trainlib import TYPES, DptAdamWArgs, call, need_gpu
+from ._trainlib import TYPES, DptAdamWArgs, Streams, call, need_gpu
 
 BLOCK = 256                # elements of a tensor that share one scale of an 8-bit state; every tensor's slot in the flat buffers is a multiple of it
 _MAX_TENSORS = 400         # per launch
@@ -100,6 +100,7 @@ class AdamW:
         self.exp_avg_scale, self.exp_avg_sq_scale = (torch.zeros(self.n_blocks, dtype=torch.float32, device=self.device) if small else None for _ in range(2))
         self._counter = torch.tensor([0.0, 1.0, 1.0, 0.0], dtype=torch.float64, device=self.device)
         self._args = self._make_args()
+        self._streams = Streams(self.device, [self._blocks, self._counter, *self._alias, *(getattr(self, n) for n in self._STATE)])
 
     # ---- flat buffers ---------------------------------------------------------------------------------------------------
     def views(self, flat: torch.Tensor):
@@ -124,6 +125,7 @@ class AdamW:
         if self.state_bits == 32:
             return self.exp_avg, self.exp_avg_sq
         m, v = torch.empty((2, self.n_blocks * BLOCK), dtype=torch.float32, device=self.device)
+        self._streams.use()
         call("dpt_adamw_moments", _trainlib.lib().dpt_adamw_moments, self.device.index, self.exp_avg.data_ptr(), self.exp_avg_scale.data_ptr(),
              self.exp_avg_sq.data_ptr(), self.exp_avg_sq_scale.data_ptr(), self.n_blocks, m.data_ptr(), v.data_ptr())
         return m, v
@@ -208,6 +210,7 @@ class AdamW:
                     raise ValueError(f"gradient {i} is {tuple(g.shape)} on {g.device}: contiguous {tuple(s)} on {self.device} is wanted")
         ptrs = list(map(_ADDRESS, grads)) if some is grads else [g.data_ptr() if g is not None else 0 for g in grads]
         L = _trainlib.lib()
+        self._streams.use()
         a = self._args
         a.grad_type = TYPES[types.pop()]
         a.lr_dev, a.lr = (self._scalar(lr, "lr"), 0.0) if isinstance(lr, torch.Tensor) else (None, self.lr if lr is None else float(lr))

@@ -271,3 +271,22 @@ def test_a_transposed_gradient_is_refused():
         with pytest.raises(ValueError):
             opt.step(bad)
     assert not p[0].any() and not p[1].any() and opt.state_dict()["step"] == 0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_an_optimiser_dropped_while_another_stream_still_works(bits):
+    """its state and records are its own memory: what is allocated after it is gone is not written over"""
+    params, opt, grads = _setup("bf16", bits, True)
+    again, opt2, _ = _setup("bf16", bits, True)
+    gs = grads()
+    opt.step(gs)
+    sizes = [t.numel() * t.element_size() for t in (opt._blocks, opt._counter, *(getattr(opt, n) for n in opt._STATE)) if t is not None]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)
+        opt2.step(gs)
+    del opt2
+    junk = [torch.zeros(n, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(params, again)) and not any(j.any() for j in junk)

@@ -397,3 +397,21 @@ def test_more_workgroups_than_one_launch_takes(long_keys):
         refs = R.attention(*args, [0, nq[-1]], [0, nk[-1]], dout=do[short:, h:h + 1])
         for got, ref, name in zip((dq, dk, dv), refs, ("dq", "dk", "dv")):
             R.within(got[short:, h:h + 1], *ref, name)
+
+
+def test_a_plan_dropped_while_another_stream_still_reads_it():
+    """the plan's offsets are the plan's own memory: what is allocated after it is gone does not overwrite what a launch under way reads (zeros there would leave
+    every complex empty)"""
+    q, k, v, do, _, plan = make([5, 40, 7], [9, 70, 3], 2, 2, 16, "f32")
+    out, stats = layers.attention_forward(q, k, v, plan)
+    ref = layers.attention_backward(do, q, k, v, out, stats, plan)
+    n, side = plan._dev.numel(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)
+        out2, stats2 = layers.attention_forward(q, k, v, plan)
+        got = layers.attention_backward(do, q, k, v, out2, stats2, plan)
+    del plan
+    junk = [torch.zeros(n, dtype=torch.int32, device="cuda") for _ in range(64)]
+    torch.cuda.synchronize()
+    assert torch.equal(out, out2) and all(torch.equal(a, b) for a, b in zip(ref[:3], got[:3])) and len(junk) == 64
