@@ -37,7 +37,14 @@ class AdamW:
     A gradient that is not finite makes its element's parameter and state NaN - with 8-bit states the state of its whole block.
 
     The step number lives on the device: a captured `step` counts on with every replay (lr and grad_scale can be device tensors for the same
-    reason).  One optimiser is used from one stream at a time."""
+    reason).  One optimiser is used from one stream at a time.
+
+    `lr` may be set between steps.  The other settings and the state buffers are fixed when the optimiser is made: the launches hold their values and
+    addresses."""
+
+    _STATE = ("master", "ema", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
+    _FIXED = ("betas", "eps", "weight_decay", "ema_decay", "state_bits") + _STATE
+    betas, eps, weight_decay, ema_decay, state_bits, master, ema, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale = (property(attrgetter("_" + n)) for n in _FIXED)
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01, no_decay: Iterable = (),
                  state_bits: int = 32, ema_decay: Optional[float] = None):
@@ -55,14 +62,14 @@ class AdamW:
         for (_, end, i), (start, _, j) in zip(spans, spans[1:]):
             if start < end:
                 raise ValueError(f"parameters {i} and {j} share memory")
-        if not lr >= 0.0 or not eps >= 0.0 or not weight_decay >= 0.0 or not all(0.0 <= b < 1.0 for b in betas):
-            raise ValueError(f"lr = {lr}, betas = {betas}, eps = {eps}, weight_decay = {weight_decay}")
+        if not eps >= 0.0 or not weight_decay >= 0.0 or not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"betas = {betas}, eps = {eps}, weight_decay = {weight_decay}")
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits = {state_bits}: 8 or 32")
         if ema_decay is not None and not 0.0 <= ema_decay <= 1.0:
             raise ValueError(f"ema_decay = {ema_decay}")
-        self.lr, self.betas, self.eps, self.weight_decay = float(lr), (float(betas[0]), float(betas[1])), float(eps), float(weight_decay)
-        self.state_bits, self.ema_decay = state_bits, ema_decay
+        self.lr, self._betas, self._eps, self._weight_decay = lr, (float(betas[0]), float(betas[1])), float(eps), float(weight_decay)
+        self._state_bits, self._ema_decay = state_bits, ema_decay
         self.params = params
         self._alias = [p.detach() for p in params]                       # keeps the updated memory alive whatever happens to the tensors
         self.dtype, self.device = params[0].dtype, params[0].device
@@ -93,14 +100,29 @@ class AdamW:
 
         def flat(dtype=torch.float32):
             return torch.zeros(self.n_blocks * BLOCK, dtype=dtype, device=self.device)
-        self.master = self._gather(flat()) if self.dtype == torch.bfloat16 else None
-        self.ema = self._gather(flat()) if ema_decay is not None else None
+        self._master = self._gather(flat()) if self.dtype == torch.bfloat16 else None
+        self._ema = self._gather(flat()) if ema_decay is not None else None
         small = state_bits == 8
-        self.exp_avg, self.exp_avg_sq = flat(torch.int8 if small else torch.float32), flat(torch.uint8 if small else torch.float32)
-        self.exp_avg_scale, self.exp_avg_sq_scale = (torch.zeros(self.n_blocks, dtype=torch.float32, device=self.device) if small else None for _ in range(2))
+        self._exp_avg, self._exp_avg_sq = flat(torch.int8 if small else torch.float32), flat(torch.uint8 if small else torch.float32)
+        self._exp_avg_scale, self._exp_avg_sq_scale = (torch.zeros(self.n_blocks, dtype=torch.float32, device=self.device) if small else None for _ in range(2))
         self._counter = torch.tensor([0.0, 1.0, 1.0, 0.0], dtype=torch.float64, device=self.device)
         self._args = self._make_args()
         self._streams = Streams(self.device, [self._blocks, self._counter, *self._alias, *(getattr(self, n) for n in self._STATE)])
+
+    @property
+    def lr(self) -> float:
+        return self._lr
+
+    @lr.setter
+    def lr(self, lr):
+        self._lr = self._rate(lr)
+
+    @staticmethod
+    def _rate(lr) -> float:
+        lr = float(lr)
+        if not lr >= 0.0:
+            raise ValueError(f"lr = {lr}")
+        return lr
 
     # ---- flat buffers ---------------------------------------------------------------------------------------------------
     def views(self, flat: torch.Tensor):
@@ -131,8 +153,6 @@ class AdamW:
         return m, v
 
     # ---- checkpoints ----------------------------------------------------------------------------------------------------
-    _STATE = ("master", "ema", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
-
     def state_dict(self):
         """Copies of the state (host-synchronising: the step number is read back)."""
         return {"step": int(self._counter[0].item()), "state_bits": self.state_bits,
@@ -213,7 +233,7 @@ class AdamW:
         self._streams.use()
         a = self._args
         a.grad_type = TYPES[types.pop()]
-        a.lr_dev, a.lr = (self._scalar(lr, "lr"), 0.0) if isinstance(lr, torch.Tensor) else (None, self.lr if lr is None else float(lr))
+        a.lr_dev, a.lr = (self._scalar(lr, "lr"), 0.0) if isinstance(lr, torch.Tensor) else (None, self._lr if lr is None else self._rate(lr))
         a.grad_scale = self._scalar(grad_scale, "grad_scale") if grad_scale is not None else None
         for i in range(0, len(ptrs), _MAX_TENSORS):
             part = array("Q", ptrs[i:i + _MAX_TENSORS])

@@ -290,3 +290,21 @@ def test_an_optimiser_dropped_while_another_stream_still_works(bits):
     junk = [torch.zeros(n, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(4)]
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(params, again)) and not any(j.any() for j in junk)
+
+
+def test_settings_that_the_launches_hold_cannot_be_set():
+    """a setting or a state buffer put in place of the optimiser's own would be ignored (or leave the launches with the address of freed memory); lr is used"""
+    opt = optim.AdamW([torch.zeros(8, device="cuda")], lr=0.5, weight_decay=0.0, ema_decay=0.5)
+    for name in ("betas", "eps", "weight_decay", "ema_decay", "state_bits", "master", "ema", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"):
+        with pytest.raises(AttributeError):
+            setattr(opt, name, torch.zeros(256, device="cuda"))
+    assert opt.betas == (0.9, 0.999) and opt.eps == 1e-8 and opt.weight_decay == 0.0 and opt.ema_decay == 0.5 and opt.state_bits == 32 and opt.master is None
+    for lr in (-1.0, float("nan")):
+        with pytest.raises(ValueError):
+            opt.lr = lr
+        with pytest.raises(ValueError):
+            opt.step([torch.ones(8, device="cuda")], lr=lr)
+    assert opt.lr == 0.5 and not opt.params[0].any() and opt.state_dict()["step"] == 0
+    opt.lr = 0.25
+    opt.step([torch.ones(8, device="cuda")])
+    assert torch.allclose(opt.params[0], torch.full((8,), -0.25, device="cuda"), rtol=1e-5)
