@@ -13,6 +13,7 @@ from typing import Iterable, Optional
 
 import numpy as np
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _trainlib
 from ._trainlib import TYPES, DptAdamWArgs, Streams, call, need_gpu
@@ -37,7 +38,8 @@ class AdamW:
     A gradient that is not finite makes its element's parameter and state NaN - with 8-bit states the state of its whole block.
 
     The step number lives on the device: a captured `step` counts on with every replay (lr and grad_scale can be device tensors for the same
-    reason).  One optimiser is used from one stream at a time.
+    reason).  One optimiser is used from one stream at a time.  A step is an in-place change of the parameters: a backward pass over activations that were
+    formed with the parameters of before raises (a replayed step moves no version counter).
 
     `lr` may be set between steps.  The other settings and the state buffers are fixed when the optimiser is made: the launches hold their values and
     addresses."""
@@ -106,8 +108,9 @@ class AdamW:
         self._exp_avg, self._exp_avg_sq = flat(torch.int8 if small else torch.float32), flat(torch.uint8 if small else torch.float32)
         self._exp_avg_scale, self._exp_avg_sq_scale = (torch.zeros(self.n_blocks, dtype=torch.float32, device=self.device) if small else None for _ in range(2))
         self._counter = torch.tensor([0.0, 1.0, 1.0, 0.0], dtype=torch.float64, device=self.device)
+        self._state = [t for t in (getattr(self, n) for n in self._STATE) if t is not None]
         self._args = self._make_args()
-        self._streams = Streams(self.device, [self._blocks, self._counter, *self._alias, *(getattr(self, n) for n in self._STATE)])
+        self._streams = Streams(self.device, [self._blocks, self._counter, *self._alias, *self._state])
 
     @property
     def lr(self) -> float:
@@ -240,6 +243,8 @@ class AdamW:
             a.tensor0, a.n_tensors, a.block0, a.last = i, len(part), self.first_block[i], int(i + len(part) == len(ptrs))
             a.n_blocks = self.first_block[i + len(part)] - a.block0
             call("dpt_adamw_step", L.dpt_adamw_step, self.device.index, C.byref(a), part.buffer_info()[0])
+        # autograd sees an in-place change, as it would of a torch operator (the aliases share the parameters' counters)
+        increment_version((self._alias if some is grads else [p for p, g in zip(self._alias, grads) if g is not None]) + self._state)
 
     def zero_grad(self):
         for p in self.params:

@@ -308,3 +308,23 @@ def test_settings_that_the_launches_hold_cannot_be_set():
     opt.lr = 0.25
     opt.step([torch.ones(8, device="cuda")])
     assert torch.allclose(opt.params[0], torch.full((8,), -0.25, device="cuda"), rtol=1e-5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_backward_pass_over_changed_parameters_raises(dtype):
+    """a step is an in-place change that autograd sees: old activations and new weights do not meet.  A parameter without a gradient is not changed"""
+    from diffphore_amd import layers
+    w, b = (torch.ones(8, dtype=T[dtype], device="cuda").requires_grad_() for _ in range(2))
+    x = torch.arange(24.0, device="cuda").view(3, 8).to(T[dtype])
+    opt = optim.AdamW([w, b], lr=0.1, ema_decay=0.5)
+    y, kept = layers.layer_norm(x, w, b), (x * b).sum()
+    opt.step([torch.ones_like(w), None])
+    assert w._version == 1 and b._version == 0 and opt.ema._version > 0
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+    kept.backward()
+    assert torch.equal(b.grad, x.sum(0))
+    layers.layer_norm(x, w, b).sum().backward()                 # the new weights' own graph
+    assert w.grad is not None
+    opt.step()
+    assert w._version == 2 and b._version == 1
