@@ -224,6 +224,15 @@ __global__ __launch_bounds__(64 * WAVES, 6) void step_kernel(DptAdamWArgs a, Gra
 #pragma unroll
         for (int e = 0; e < 4; ++e) x.ev[e] = x.ev[e] * ema_d + x.pv[e] * ema_o;
       }
+      if (x.b.left < BLOCK) {                                // what pads a tensor's last block stays 0 whatever the factors are (eps 0: 0 / 0; an infinite scale)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (lane * 4 + e < x.b.left) continue;
+          x.pv[e] = 0.f;
+          if constexpr (EMA) x.ev[e] = 0.f;
+          if constexpr (BITS == 32) x.mv[e] = x.vv[e] = 0.f;
+        }
+      }
       // the next block's values are waited for here, before the stores: loads and stores share a counter, and a wait behind the stores would be one for them too
       __builtin_amdgcn_s_waitcnt(0x0f70);                    // vmcnt(0)
       if constexpr (BITS == 32) {

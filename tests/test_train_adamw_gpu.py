@@ -328,3 +328,23 @@ def test_a_backward_pass_over_changed_parameters_raises(dtype):
     assert w.grad is not None
     opt.step()
     assert w._version == 2 and b._version == 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_padding_stays_zero_whatever_the_factors(dtype, bits):
+    """what fills a tensor's last block up is 0 in every flat buffer: also without eps (0 / 0 there) and with a gradient scale or a learning rate of infinity"""
+    inf = torch.tensor(float("inf"), device="cuda")
+    for eps, kw in ((0.0, {}), (1e-8, dict(grad_scale=inf)), (1e-8, dict(lr=inf)), (0.0, dict(grad_scale=torch.zeros_like(inf)))):
+        params, _, grads = _setup(dtype, bits, False)
+        opt = optim.AdamW(params, lr=LR, eps=eps, state_bits=bits, ema_decay=D)
+        gs = grads()
+        gs[3] = None                                                     # a tensor that is left alone
+        opt.step(gs, **kw)
+        flats = [f for f in (opt.master, opt.ema, opt.exp_avg, opt.exp_avg_sq) if f is not None]
+        assert len(flats) == (4 if dtype == "bf16" else 3)
+        for f in flats:
+            for lo, hi, n in zip(opt.first_block, opt.first_block[1:], opt._numel):
+                assert not f[lo * 256 + n:hi * 256].float().ne(0).any(), (eps, kw)
+        if not kw:
+            assert all(torch.isfinite(p).all() for p in params) and torch.isfinite(opt.ema).all()
