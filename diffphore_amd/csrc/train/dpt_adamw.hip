@@ -38,8 +38,9 @@ __device__ __forceinline__ float wave_max(float x) {
 }
 
 // Position t = TOP (x / scale)^(1/POW) of a value on its curve.  x (rounded from 64 bits) and its product with 1 / scale are good to 2^-24, 1 / scale and a root
-// to an ulp, so |dt| < TOP 2^-24 (4 / POW + 3) < 8e-5 on both curves (NEAR); below TINY the 32-bit values may have lost bits to underflow.
-constexpr float NEAR = 1e-4f, TINY = 1e-30f;
+// to an ulp, so |dt| < TOP 2^-24 (4 / POW + 3) < 8e-5 on both curves (NEAR); below TINY the 32-bit values may have lost bits to underflow, and
+// above VAST 1 / scale is (the hardware's reciprocal of more than 2^126 is 0): such blocks take the 64-bit codes.
+constexpr float NEAR = 1e-4f, TINY = 1e-30f, VAST = 0x1p125f;
 template <int TOP, int POW>
 __device__ __forceinline__ float position(float x, float inv) {
   float t = __builtin_amdgcn_sqrtf(x * inv);
@@ -182,9 +183,9 @@ __global__ __launch_bounds__(64 * WAVES, 6) void step_kernel(DptAdamWArgs a, Gra
         if (__any(bad != 0.f)) {
           msc = vsc = __builtin_nanf("");
         } else {
-          const float mi = __builtin_amdgcn_rcpf(msc), vi = __builtin_amdgcn_rcpf(vsc);       // not used below TINY
+          const float mi = __builtin_amdgcn_rcpf(msc), vi = __builtin_amdgcn_rcpf(vsc);       // not used below TINY and above VAST
           int cm[4], cv[4];
-          int near = (msc < TINY) | (vsc < TINY);
+          int near = (msc < TINY) | (vsc < TINY) | (msc > VAST) | (vsc > VAST);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float tm = position<127, 2>(fabsf(x.mv[e]), mi), tv = position<255, 4>(x.vv[e], vi);

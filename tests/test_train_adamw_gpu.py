@@ -348,3 +348,19 @@ def test_padding_stays_zero_whatever_the_factors(dtype, bits):
                 assert not f[lo * 256 + n:hi * 256].float().ne(0).any(), (eps, kw)
         if not kw:
             assert all(torch.isfinite(p).all() for p in params) and torch.isfinite(opt.ema).all()
+
+
+@pytest.mark.parametrize("top", [4e20, 2.9e20, 2e20, 3e19])
+def test_codes_of_the_largest_second_moments(top):
+    """v up to the last values before overflow, where 1 / v is below the normal 32-bit numbers: the codes are those of the formula in 64 bits there, too"""
+    g = torch.Generator().manual_seed(3)
+    grad = torch.randn(1000, generator=g) * (top / 4)
+    grad[5] = top
+    grad[300:] *= 1e-3                                                   # blocks of ordinary scales beside it
+    p = torch.zeros(1000, device="cuda")
+    opt = optim.AdamW([p], lr=1e-3, betas=(0.9, 0.999), weight_decay=0.0, state_bits=8)
+    opt.step([grad.cuda()])
+    x = torch.nn.functional.pad(grad.double(), (0, 24))
+    for val, power, code, scale in ((x * (1 - 0.9), 2, opt.exp_avg, opt.exp_avg_scale), (x * x * (1 - 0.999), 4, opt.exp_avg_sq, opt.exp_avg_sq_scale)):
+        want, s = R.encode(val, power)
+        assert torch.equal(scale.cpu(), s) and torch.equal(code.cpu(), want), power
