@@ -156,7 +156,7 @@ __global__ __launch_bounds__(64 * WAVES, 6) void step_kernel(DptAdamWArgs a, Gra
         for (int e = 0; e < 4; ++e) {
           const float g = (float)x.gv[e] * gs;
           x.mv[e] = x.mv[e] * b1 + g * omb1;
-          x.vv[e] = x.vv[e] * b2 + g * g * omb2;
+          x.vv[e] = x.vv[e] * b2 + g * omb2 * g;             // (in this order g^2, which may pass the 32-bit numbers where v does not, is never formed)
         }
       } else {
         const double ma = (double)x.ms, va = (double)x.vs;
@@ -214,10 +214,11 @@ __global__ __launch_bounds__(64 * WAVES, 6) void step_kernel(DptAdamWArgs a, Gra
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        // root and quotient to an ulp each, of an update that is itself a small part of the parameter; moments next to underflow are rooted 2^64 times as large
+        // root and quotient to an ulp each, of an update that is itself a small part of the parameter; moments next to underflow are rooted 2^64 times as large,
+        // those next to overflow (v / (1 - b2^t) may pass it where v does not) 2^64 times as small
         const float w = x.vv[e] * ic2;
-        const bool tiny = w < 0x1p-96f;
-        const float root = __builtin_amdgcn_sqrtf(tiny ? w * 0x1p64f : w), den = (tiny ? root * 0x1p-32f : root) + eps;
+        const bool tiny = w < 0x1p-96f, vast = w > 0x1p96f;
+        const float root = __builtin_amdgcn_sqrtf(tiny ? w * 0x1p64f : vast ? x.vv[e] * 0x1p-64f * ic2 : w), den = root * (tiny ? 0x1p-32f : vast ? 0x1p32f : 1.f) + eps;
         const float q = x.mv[e] * __builtin_amdgcn_rcpf(den);
         x.pv[e] = fmaf(-lr1, q, x.pv[e] * shrink);
       }

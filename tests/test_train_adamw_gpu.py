@@ -364,3 +364,18 @@ def test_codes_of_the_largest_second_moments(top):
     for val, power, code, scale in ((x * (1 - 0.9), 2, opt.exp_avg, opt.exp_avg_scale), (x * x * (1 - 0.999), 4, opt.exp_avg_sq, opt.exp_avg_sq_scale)):
         want, s = R.encode(val, power)
         assert torch.equal(scale.cpu(), s) and torch.equal(code.cpu(), want), power
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_updates_of_the_largest_second_moments(bits):
+    """v / (1 - b2^t) = g^2 passes the 32-bit numbers at g = 1.8e19, v itself only at 5.8e20: the first step is lr in every direction up to there"""
+    grad = torch.tensor([1.0, 1e10, -1e15, 1e19, 2e19, 1e20, -4e20, 5e20])
+    p = torch.zeros(8, device="cuda")
+    opt = optim.AdamW([p], lr=1.0, betas=(0.9, 0.999), weight_decay=0.0, state_bits=bits)
+    opt.step([grad.cuda()])
+    # m / c1 and v / c2 are g and g^2 to a few roundings
+    assert torch.allclose(p.cpu(), -grad.sign(), rtol=1e-5)
+    if bits == 32:
+        opt.step([torch.zeros(8, device="cuda")])
+        m, v = 0.9 * 0.1 / (1 - 0.81), 0.999 * 0.001 / (1 - 0.999 ** 2)
+        assert torch.allclose(p.cpu(), -grad.sign() * (1 + m / v ** 0.5), rtol=1e-5)
