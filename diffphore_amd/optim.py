@@ -20,7 +20,7 @@ from ._trainlib import TYPES, DptAdamWArgs, Streams, call, need_gpu
 
 BLOCK = 256                # elements of a tensor that share one scale of an 8-bit state; every tensor's slot in the flat buffers is a multiple of it
 _MAX_TENSORS = 400         # per launch
-_DTYPE, _NUMEL, _DEVICE, _CONTIGUOUS, _ADDRESS = attrgetter("dtype"), torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous, torch.Tensor.data_ptr
+_DTYPE, _SHAPE, _DEVICE, _CONTIGUOUS, _ADDRESS = attrgetter("dtype"), attrgetter("shape"), torch.Tensor.get_device, torch.Tensor.is_contiguous, torch.Tensor.data_ptr
 _RECORD = np.dtype([("param", "u8"), ("tensor", "i4"), ("index", "i4"), ("left", "i4"), ("decay", "f4"), ("pad", "i4", 2)])
 
 
@@ -82,8 +82,6 @@ class AdamW:
                 raise ValueError(f"no_decay: there is no parameter {n!r}")
             decay[number[n] if number is not None else int(n)] = 0.0
         self._numel, self._sizes = [p.numel() for p in params], [p.shape for p in params]
-        self._matrices = [i for i, s in enumerate(self._sizes) if len(s) > 1]
-        self._matrix_sizes = [self._sizes[i] for i in self._matrices]
         blocks = [-(-n // BLOCK) for n in self._numel]
         self.first_block = [0]
         for b in blocks:
@@ -222,11 +220,7 @@ class AdamW:
         types = set(map(_DTYPE, some)) or {self.dtype}
         if len(types) > 1 or not types <= {self.dtype, torch.float32}:
             raise TypeError(f"gradients in {types}: all in {self.dtype}, or all in float32")
-        if some is grads:
-            # element counts of all, shapes of the matrices: a vector's gradient with the right count lies as the vector does, whatever its shape
-            fits = list(map(_NUMEL, grads)) == self._numel and [grads[i].shape for i in self._matrices] == self._matrix_sizes
-        else:
-            fits = [g.shape for g in some] == [s for s, g in zip(self._sizes, grads) if g is not None]
+        fits = list(map(_SHAPE, some)) == (self._sizes if some is grads else [s for s, g in zip(self._sizes, grads) if g is not None])
         if not fits or not set(map(_DEVICE, some)) <= {self.device.index} or not all(map(_CONTIGUOUS, some)):
             for i, (g, s) in enumerate(zip(grads, self._sizes)):
                 if g is not None and (g.shape != s or g.get_device() != self.device.index or not g.is_contiguous()):

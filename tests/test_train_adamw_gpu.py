@@ -379,3 +379,18 @@ def test_updates_of_the_largest_second_moments(bits):
         opt.step([torch.zeros(8, device="cuda")])
         m, v = 0.9 * 0.1 / (1 - 0.81), 0.999 * 0.001 / (1 - 0.999 ** 2)
         assert torch.allclose(p.cpu(), -grad.sign() * (1 + m / v ** 0.5), rtol=1e-5)
+
+
+def test_gradients_have_their_parameters_shapes():
+    """one rule, whether or not some gradients are None"""
+    p = [torch.zeros(4, 6, device="cuda"), torch.zeros(5, device="cuda"), torch.zeros((), device="cuda")]
+    opt = optim.AdamW(p)
+    good = [torch.ones_like(t) for t in p]
+    for i, shape in ((0, (24,)), (0, (6, 4)), (1, (5, 1)), (1, (1, 5)), (2, (1,))):
+        for rest in (good, [None] * 3):
+            with pytest.raises(ValueError, match=f"gradient {i}"):
+                opt.step([torch.ones(shape, device="cuda") if j == i else g for j, g in enumerate(rest)])
+    assert opt.state_dict()["step"] == 0 and not any(t.any() for t in p)
+    opt.step(good)
+    opt.step([None, good[1], None])
+    assert opt.state_dict()["step"] == 2 and all(t.any() for t in p)
