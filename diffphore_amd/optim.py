@@ -155,8 +155,8 @@ class AdamW:
 
     # ---- checkpoints ----------------------------------------------------------------------------------------------------
     def state_dict(self):
-        """Copies of the state (host-synchronising: the step number is read back)."""
-        return {"step": int(self._counter[0].item()), "state_bits": self.state_bits,
+        """Copies of the state, with the names and shapes of the tensors that it belongs to (host-synchronising: the step number is read back)."""
+        return {"step": int(self._counter[0].item()), "state_bits": self.state_bits, "names": list(self.names) if self.names is not None else None, "sizes": [tuple(s) for s in self._sizes],
                 **{n: getattr(self, n).clone() if getattr(self, n) is not None else None for n in self._STATE}}
 
     def _refresh(self):
@@ -166,12 +166,18 @@ class AdamW:
             p.copy_(m)
 
     def load_state_dict(self, state):
-        """The state of `state_dict`; bf16 parameters become the roundings of the loaded masters (fp32 parameters are not part of the state)."""
+        """The state of `state_dict`, of an optimiser of the same tensors in the same order (a state without `names` or `sizes` is taken by the length of its
+        buffers); bf16 parameters become the roundings of the loaded masters (fp32 parameters are not part of the state)."""
         t = int(state["step"])
         if t < 0:
             raise ValueError(f"step = {t}")
         if state["state_bits"] != self.state_bits:
             raise ValueError(f"the state has {state['state_bits']} bits, the optimiser {self.state_bits}")
+        names, sizes = state.get("names"), state.get("sizes")
+        if sizes is not None and [tuple(s) for s in sizes] != [tuple(s) for s in self._sizes]:
+            raise ValueError("the state belongs to tensors of other shapes, or in another order")
+        if names is not None and self.names is not None and list(names) != self.names:
+            raise ValueError("the state belongs to tensors of other names, or in another order")
         for n in self._STATE:
             mine, given = getattr(self, n), state.get(n)
             if (mine is None) != (given is None) or (mine is not None and (mine.shape != given.shape or mine.dtype != given.dtype)):

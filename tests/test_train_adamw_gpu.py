@@ -394,3 +394,21 @@ def test_gradients_have_their_parameters_shapes():
     opt.step(good)
     opt.step([None, good[1], None])
     assert opt.state_dict()["step"] == 2 and all(t.any() for t in p)
+
+
+def test_a_state_of_other_tensors_is_refused():
+    """buffers of the same length whose tensors lie in another order, have other shapes or other names"""
+    make = lambda **kw: optim.AdamW({n: torch.zeros(s, device="cuda") for n, s in kw.items()})                             # noqa: E731
+    opt = make(a=(300,), b=(20, 20))
+    opt.step({"a": torch.ones(300, device="cuda"), "b": torch.full((20, 20), 2.0, device="cuda")})
+    state = opt.state_dict()
+    for other in (make(b=(20, 20), a=(300,)), make(a=(300,), b=(400,)), make(a=(300,), c=(20, 20)), make(a=(301,), b=(20, 20)), make(a=(512,), b=(512,))):
+        with pytest.raises(ValueError):
+            other.load_state_dict(state)
+        assert not other.exp_avg.any() and other.state_dict()["step"] == 0
+    for same in (make(a=(300,), b=(20, 20)), optim.AdamW([torch.zeros(300, device="cuda"), torch.zeros(20, 20, device="cuda")])):
+        same.load_state_dict(state)
+        assert torch.equal(same.exp_avg, opt.exp_avg) and same.state_dict()["step"] == 1
+    again = make(a=(300,), b=(20, 20))
+    again.load_state_dict({n: t for n, t in state.items() if n not in ("names", "sizes")})
+    assert torch.equal(again.exp_avg_sq, opt.exp_avg_sq)
