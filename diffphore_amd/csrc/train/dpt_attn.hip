@@ -10,7 +10,8 @@ size_t up(size_t n) { return (n + ALIGN - 1) / ALIGN * ALIGN; }
 
 int check(const DptAttnArgs* a) {
   if (!a || (a->type != DPT_F32 && a->type != DPT_BF16)) return DPT_E_BADARG;
-  if (a->B < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->dim < 1 || !(a->scale > 0.f) || a->scale > 3.4e38f) return DPT_E_BADARG;
+  if (a->B < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->dim < 1) return DPT_E_BADARG;
+  if (!(a->scale >= 0x1p-126f && a->scale <= 0x1p126f)) return DPT_E_BADARG;             // scale log2 e has to be a normal number
   if (a->n_q < 0 || a->n_k < 0 || a->max_nq < 0 || a->max_nk < 0 || a->max_nq > a->n_q || a->max_nk > a->n_k || a->n_pairs < 0 || a->splits < 0) return DPT_E_BADARG;
   if (a->dim > 128 || a->n_q > MOST_ROWS || a->n_k > MOST_ROWS) return DPT_E_TOOLARGE;   // the last block's row numbers, past the end, still fit
   const int64_t group = a->heads / a->kv_heads, rows = (int64_t)a->max_nq * group;

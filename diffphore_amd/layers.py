@@ -205,8 +205,8 @@ def _check_attn(q, k, v, plan, bias, scale):
         raise ValueError(f"head dimension {dim}: 1 to 128 are supported")
     if q.shape[0] != plan.n_q or k.shape[0] != plan.n_k:
         raise ValueError(f"{q.shape[0]} query and {k.shape[0]} key rows, the plan has {plan.n_q} and {plan.n_k}")
-    if not (0.0 < scale < 3e38):
-        raise ValueError(f"scale = {scale}: a positive finite number is wanted")
+    if not 2.0 ** -126 <= scale <= 2.0 ** 126:
+        raise ValueError(f"scale = {scale}: a positive number from 2^-126 to 2^126 is wanted")
     if bias is not None:
         need_gpu(bias, "bias")
         if bias.shape != (heads, plan.n_pairs) or bias.dtype != q.dtype or bias.device != q.device:

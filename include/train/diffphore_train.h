@@ -63,7 +63,7 @@ typedef struct DptAttnArgs {
   int32_t n_q, n_k;                /* rows of q and k */
   int32_t max_nq, max_nk;          /* largest complex */
   int64_t n_pairs;
-  float scale;                     /* > 0 */
+  float scale;                     /* 2^-126 .. 2^126 */
   int32_t splits;                  /* ranges of keys (backward: of rows, too) per workgroup that are joined afterwards, up to 64; 0 = chosen by the library */
   /* strides in elements; the last dimension has unit stride */
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, dout_row, dout_head, bias_head, bias_pair;

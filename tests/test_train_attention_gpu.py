@@ -415,3 +415,18 @@ def test_a_plan_dropped_while_another_stream_still_reads_it():
     junk = [torch.zeros(n, dtype=torch.int32, device="cuda") for _ in range(64)]
     torch.cuda.synchronize()
     assert torch.equal(out, out2) and all(torch.equal(a, b) for a, b in zip(ref[:3], got[:3])) and len(junk) == 64
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_the_smallest_and_largest_scales(dtype):
+    """scales whose exponent factor is no normal number are refused; at the ends of the range equal scores still weigh equally"""
+    v = torch.randn(4, 1, 8, generator=torch.Generator().manual_seed(1)).to(T[dtype]).cuda()
+    plan = layers.PairPlan([0, 4], [0, 4])
+    for scale in (1e-50, 1e-39, 1e38, 2.9e38, 1e300):
+        with pytest.raises(ValueError, match="scale"):
+            layers.attention_forward(v, v, v, plan, scale=scale)
+    for scale, q in ((2.0 ** -126, v), (2.0 ** 126, torch.zeros_like(v))):
+        out, stats = layers.attention_forward(q, q, v, plan, scale=scale)
+        (o, bo), _, (l, bl) = R.attention(q, q, v, [0, 4], [0, 4], scale=scale)
+        R.within(out, o, bo, "out")
+        R.within(stats[1], l, bl, "l")

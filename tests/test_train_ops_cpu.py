@@ -162,3 +162,12 @@ def test_lengths_and_counts_whose_arithmetic_would_wrap_are_too_large(kw):
     assert L.dpt_attn_fwd(C.byref(a), None) == -1
     with pytest.raises(ValueError, match="rows"):
         layers.PairPlan([0, 1], [0, 2 ** 31 - 1024])
+
+
+@pytest.mark.parametrize("scale", [1e-39, -1.0, 2.9e38, float("inf"), 2.0 ** 126])
+def test_scales_without_a_normal_exponent_factor_are_refused(scale):
+    """the kernels form scale log2 e: 0 or infinite, it made rows of equal scores NaN (the pointers are NULL and valid scales end at those: both -1)"""
+    L = _trainlib.lib()
+    ok = scale == 2.0 ** 126
+    a = _attn_args(scale=scale)
+    assert (L.dpt_attn_ws_bytes(C.byref(a), 1) > 0) == ok and L.dpt_attn_fwd(C.byref(a), None) == -1
