@@ -96,6 +96,7 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     x2, dy2 = _rows(x), _rows(dy)
     rows, width = x2.shape
     for t, name in ((mean, "mean"), (rstd, "rstd")):
+        need_gpu(t, name)
         if t.dtype != torch.float32 or t.numel() != rows or t.device != x.device or not t.is_contiguous():
             raise ValueError(f"{name}: {rows} contiguous float32 values on {x.device} are wanted (layer_norm_forward's)")
     wtype = weight.dtype if weight is not None else param_dtype or x.dtype
@@ -194,6 +195,8 @@ def _check_attn(q, k, v, plan, bias, scale):
             raise ValueError(f"{name} has shape {tuple(t.shape)}: [rows, heads, dim] is wanted")
         if t.dtype is not q.dtype or t.get_device() != q.get_device():
             raise ValueError(f"{name} is {t.dtype} on {t.device}, q is {q.dtype} on {q.device}")
+    if not isinstance(plan, PairPlan):
+        raise TypeError(f"plan: a PairPlan is wanted, got {type(plan).__name__}")
     if plan.device.index != q.get_device():
         raise ValueError(f"the plan is on {plan.device}, q on {q.device}")
     heads, dim = q.shape[1:]
@@ -267,6 +270,7 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
         need_gpu(t, name)
         if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
             raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}, q is {tuple(q.shape)} {q.dtype} on {q.device}")
+    need_gpu(stats, "stats")
     if stats.shape != (2, q.shape[1], q.shape[0]) or stats.dtype != torch.float32 or stats.device != q.device:
         raise ValueError(f"stats is {tuple(stats.shape)} {stats.dtype} on {stats.device}: attention_forward's is wanted")
     L = _trainlib.lib()

@@ -201,6 +201,8 @@ class AdamW:
         return a
 
     def _scalar(self, x, name):
+        if not isinstance(x, torch.Tensor):
+            raise TypeError(f"{name}: a tensor is wanted, got {type(x).__name__}")
         if x.dtype != torch.float32 or x.numel() != 1 or x.device != self.device:
             raise ValueError(f"{name}: one float32 value on {self.device} is wanted, got {x.numel()} of {x.dtype} on {x.device}")
         return x.data_ptr()

@@ -168,3 +168,21 @@ def test_averaged_weights_drive_the_score_model():
     model = TensorProductScoreModel(device="cuda:0").load_state_dict(averaged)
     for a, b in zip(model(batch), ref):                                                    # the score model's own bound (test_forward_gpu.py)
         assert (a.double().cpu() - b.double().cpu()).abs().max() < 1e-5 * b.abs().max()
+
+
+def test_what_is_no_tensor_or_plan_is_a_type_error():
+    x = torch.zeros(2, 8, device="cuda")
+    q = torch.zeros(2, 1, 8, device="cuda")
+    plan = layers.PairPlan([0, 2], [0, 2])
+    _, mean, rstd = layers.layer_norm_forward(x)
+    out, stats = layers.attention_forward(q, q, q, plan)
+    opt = optim.AdamW([x.clone()])
+    for call in (lambda: layers.layer_norm_backward(x, x, None, rstd), lambda: layers.layer_norm_backward(x, x, mean, 1.0), lambda: layers.layer_norm_backward(None, x, mean, rstd),
+                 lambda: layers.attention_backward(q, q, q, q, out, None, plan), lambda: layers.attention_backward(q, q, q, q, None, stats, plan),
+                 lambda: layers.attention_forward(q, q, q, None), lambda: layers.attention_forward(q, q, q, ([0, 2], [0, 2])), lambda: opt.step([x], grad_scale=0.5)):
+        with pytest.raises(TypeError):
+            call()
+    for call in (lambda: layers.layer_norm_backward(x, x, mean.cpu(), rstd), lambda: layers.attention_backward(q, q, q, q, out, stats.cpu(), plan)):
+        with pytest.raises(ValueError):
+            call()
+    assert opt.state_dict()["step"] == 0
