@@ -199,7 +199,8 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void fwd_kernel(D
   if (!rb.live) return;
   // the sum in terms of the true maximum
   l = half_sum(l);
-  const float lm = m == NEG_INF ? 0.f : l * __builtin_amdgcn_exp2f((base - m) * c), mm = FAST<T, BIAS> ? m * d.a.scale : m;
+  if (l == 0.f) zero<DP / 32>(o);                            // a row that sees nothing: 0, also beside values that are not finite (a NaN row has l = NaN)
+  const float lm = m == NEG_INF ? l : l * __builtin_amdgcn_exp2f((base - m) * c), mm = FAST<T, BIAS> ? m * d.a.scale : m;
   const int64_t at = row.token * d.a.heads + row.head, st = (int64_t)row.head * d.a.n_q + row.token, plane = (int64_t)d.a.heads * d.a.n_q;
   if (d.splits == 1) {
     store_col<T, DP, VEC>((T*)d.a.out + at * d.a.dim, h, d.a.dim, o, l == 0.f ? 0.f : 1.f / l);
@@ -251,6 +252,7 @@ struct Probs {
       f1 = l == 0.f ? 0.f : 1.f / l;
     }
   }
+  __device__ __forceinline__ bool nothing() const { return FAST<T, BIAS> ? f0 == NEG_INF : f1 == 0.f; }    // the row sees no key
   static __device__ __forceinline__ float p(float x, float c, float f0, float f1) {
     return FAST<T, BIAS> ? __builtin_amdgcn_exp2f(fmaf(x, c, f0)) : __builtin_amdgcn_exp2f((x - f0) * c) * f1;
   }
@@ -380,6 +382,7 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dq_kernel(De
     work(kt1, vt1, t + 1);
   }
   if (!rb.live) return;
+  if (f.nothing()) zero<DP / 32>(dq);
   if (d.splits_q == 1) store_col<T, DP, VEC>((T*)d.a.dq + at * d.a.dim, h, d.a.dim, dq, d.a.scale);
   else store_col<float, DP, VEC>(d.part_g + (split * plane + at) * d.a.dim, h, d.a.dim, dq, d.a.scale);
   if (h == 0 && split == 0) {

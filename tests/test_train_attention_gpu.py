@@ -430,3 +430,24 @@ def test_the_smallest_and_largest_scales(dtype):
         (o, bo), _, (l, bl) = R.attention(q, q, v, [0, 4], [0, 4], scale=scale)
         R.within(out, o, bo, "out")
         R.within(stats[1], l, bl, "l")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("nk", [40, 3000])
+def test_rows_without_keys_are_zero_beside_values_that_are_not_finite(nk, dtype):
+    """out and dq of a row that sees nothing are 0 whatever k and v hold; a row that is NaN itself is no such row, and its statistics say so"""
+    q, k, v, do, _, plan = make([nk + 3], [nk], 1, 1, 32, dtype)                         # causal: the first 3 rows see nothing
+    q[8, 0, 1] = math.nan
+    k[0], v[0] = math.nan, math.inf                                                      # in the tile of the first rows
+    out, stats = layers.attention_forward(q, k, v, plan, causal=True)
+    assert not out[:3].any() and (stats[0, 0, :3] == -math.inf).all() and not stats[1, 0, :3].any()
+    assert torch.isnan(out[8]).all() and torch.isnan(stats[1, 0, 8])
+    dq = layers.attention_backward(do, q, k, v, out, stats, plan, causal=True)[0]
+    assert not dq[:3].any() and torch.isnan(dq[8]).all()
+    q, k, v, do, b, plan = make([3], [nk], 1, 1, 32, dtype, True)                        # (3000 keys: ranges that are joined)
+    b.view(1, 3, nk)[:, 1] = -math.inf
+    k[nk - 1], v[nk - 1] = math.inf, math.nan
+    out, stats = layers.attention_forward(q, k, v, plan, bias=b)
+    assert not out[1].any() and not stats[1, 0, 1] and torch.isnan(out[0]).all()
+    dq, _, _, db = layers.attention_backward(do, q, k, v, out, stats, plan, bias=b)
+    assert not dq[1].any()
