@@ -412,3 +412,31 @@ def test_a_state_of_other_tensors_is_refused():
     again = make(a=(300,), b=(20, 20))
     again.load_state_dict({n: t for n, t in state.items() if n not in ("names", "sizes")})
     assert torch.equal(again.exp_avg_sq, opt.exp_avg_sq)
+
+
+@pytest.mark.parametrize("dtype, bits", [("f32", 32), ("bf16", 8)])
+def test_every_launch_of_a_long_list_follows_the_formula(dtype, bits):
+    """900 tensors take three launches: parameters, moments and averages of each, and the tensors without decay, against the formula"""
+    sizes = [(i % 5 + 1,) if i % 90 else (300 + i,) for i in range(900)]
+    free = (0, 4, 399, 400, 450, 801, 899)
+    g = torch.Generator().manual_seed(6)
+    params = [torch.randn(s, generator=g).to(T[dtype]).cuda() for s in sizes]
+    grads = [(torch.randn(s, generator=g) * 10.0 ** (i % 4 - 2)).to(T[dtype]).cuda() for i, s in enumerate(sizes)]
+    before = [p.double().cpu() for p in params]
+    opt = optim.AdamW(params, lr=LR, betas=(B1, B2), eps=EPS, weight_decay=WD, no_decay=free, state_bits=bits, ema_decay=D)
+    opt.step(grads)
+    for i, p in enumerate(params):
+        z = torch.zeros(sizes[i], dtype=torch.float64)
+        (pr, bp), (mr, bm), (vr, bv) = R.adamw(before[i], grads[i], z, z, 1, LR, B1, B2, EPS, 0.0 if i in free else WD)
+        new = (opt.views(opt.master)[i] if dtype == "bf16" else p).double().cpu()
+        R.within(new, pr, bp, f"p{i}")
+        assert torch.equal(p.cpu(), new.to(T[dtype]))
+        R.within(opt.views(opt.ema)[i], D * before[i] + (1 - D) * new, 4 * R.F32 * (before[i].abs() + new.abs()), f"ema{i}")
+        if bits == 32:
+            R.within(opt.views(opt.exp_avg)[i], mr, bm, f"m{i}")
+            R.within(opt.views(opt.exp_avg_sq)[i], vr, bv, f"v{i}")
+        else:
+            for x, power, code, scale in ((mr, 2, opt.exp_avg, opt.exp_avg_scale), (vr, 4, opt.exp_avg_sq, opt.exp_avg_sq_scale)):
+                c, s = R.encode(torch.nn.functional.pad(x, (0, -len(x) % 256)), power)
+                lo, hi = opt.first_block[i], opt.first_block[i + 1]
+                assert torch.equal(code[lo * 256:hi * 256].cpu(), c) and torch.allclose(scale[lo:hi].cpu(), s, rtol=2.0 ** -23, atol=0), (i, power)

@@ -451,3 +451,12 @@ def test_rows_without_keys_are_zero_beside_values_that_are_not_finite(nk, dtype)
     assert not out[1].any() and not stats[1, 0, 1] and torch.isnan(out[0]).all()
     dq, _, _, db = layers.attention_backward(do, q, k, v, out, stats, plan, bias=b)
     assert not dq[1].any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("causal", [False, True])
+def test_a_complex_alone_holds_the_same_bounds(causal, dtype):
+    """alone or in a batch, a complex's rows are those of the definition; their bits may differ, since the number of joined ranges goes by the batch"""
+    q, k, v, do, b, plan = make([200, 31], [333, 64], 4, 2, 64, dtype, True)
+    check(q, k, v, do, b, plan, causal=causal)
+    check(q[200:], k[333:], v[333:], do[200:], b[:, 200 * 333:], layers.PairPlan([0, 31], [0, 64]), causal=causal)

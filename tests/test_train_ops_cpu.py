@@ -171,3 +171,23 @@ def test_scales_without_a_normal_exponent_factor_are_refused(scale):
     ok = scale == 2.0 ** 126
     a = _attn_args(scale=scale)
     assert (L.dpt_attn_ws_bytes(C.byref(a), 1) > 0) == ok and L.dpt_attn_fwd(C.byref(a), None) == -1
+
+
+@pytest.mark.parametrize("power", [2, 4])
+def test_decoded_codes_are_finite_and_a_block_of_zeros_stays_zero(power):
+    g = torch.Generator().manual_seed(power)
+    x = torch.randn(4 * 256, generator=g, dtype=torch.float64) * torch.exp(4 * torch.randn(4 * 256, generator=g, dtype=torch.float64))
+    x = x.abs() if power == 4 else x
+    x[256:512] = 0
+    code, scale = R.encode(x, power)
+    y = R.decode(code, scale, power)
+    assert torch.isfinite(y).all() and not code[256:512].any() and not y[256:512].any()
+    # off by half a step of the curve's axis, or by less than a step where a second moment is kept from becoming 0
+    top = 127 if power == 2 else 255
+    root = lambda t: (t.abs().view(-1, 256) / scale.double()[:, None].clamp(min=1e-300)) ** (1 / power) * top              # noqa: E731
+    off = (root(x) - root(y)).abs()
+    kept = (root(x) < 0.5) & (root(x) > 0)
+    if power == 4:
+        assert (code.view(-1, 256)[kept] == 1).all() and off[kept].max() < 1
+        off = off[~kept]
+    assert off.max() <= 0.5 + 1e-5
