@@ -382,7 +382,13 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dq_kernel(De
     work(kt1, vt1, t + 1);
   }
   if (!rb.live) return;
-  if (f.nothing()) zero<DP / 32>(dq);
+  // a row that sees nothing: 0, also beside keys that are not finite (a branch around zero() costs the bf16 kernel of 64 dimensions five registers and its third
+  // wave per SIMD: 55 -> 64 us for 48 ragged complexes of up to 700 x 900)
+  const bool none = f.nothing();
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dq[i][e] = none ? 0.f : dq[i][e];
   if (d.splits_q == 1) store_col<T, DP, VEC>((T*)d.a.dq + at * d.a.dim, h, d.a.dim, dq, d.a.scale);
   else store_col<float, DP, VEC>(d.part_g + (split * plane + at) * d.a.dim, h, d.a.dim, dq, d.a.scale);
   if (h == 0 && split == 0) {
