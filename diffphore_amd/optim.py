@@ -20,7 +20,7 @@ from ._trainlib import TYPES, DptAdamWArgs, Streams, call, need_gpu
 
 BLOCK = 256                # elements of a tensor that share one scale of an 8-bit state; every tensor's slot in the flat buffers is a multiple of it
 _MAX_TENSORS = 400         # per launch
-_DTYPE, _SHAPE, _DEVICE, _CONTIGUOUS, _ADDRESS = attrgetter("dtype"), attrgetter("shape"), torch.Tensor.get_device, torch.Tensor.is_contiguous, torch.Tensor.data_ptr
+_DTYPE, _SHAPE, _DEVICE, _CONTIGUOUS, _ADDRESS = attrgetter("dtype"), torch.Tensor.size, torch.Tensor.get_device, torch.Tensor.is_contiguous, torch.Tensor.data_ptr
 _RECORD = np.dtype([("param", "u8"), ("tensor", "i4"), ("index", "i4"), ("left", "i4"), ("decay", "f4"), ("pad", "i4", 2)])
 
 
@@ -107,6 +107,7 @@ class AdamW:
         self._exp_avg_scale, self._exp_avg_sq_scale = (torch.zeros(self.n_blocks, dtype=torch.float32, device=self.device) if small else None for _ in range(2))
         self._counter = torch.tensor([0.0, 1.0, 1.0, 0.0], dtype=torch.float64, device=self.device)
         self._state = [t for t in (getattr(self, n) for n in self._STATE) if t is not None]
+        self._changed = self._alias + self._state
         self._args = self._make_args()
         self._streams = Streams(self.device, [self._blocks, self._counter, *self._alias, *self._state])
 
@@ -246,7 +247,7 @@ class AdamW:
             a.n_blocks = self.first_block[i + len(part)] - a.block0
             call("dpt_adamw_step", L.dpt_adamw_step, self.device.index, C.byref(a), part.buffer_info()[0])
         # autograd sees an in-place change, as it would of a torch operator (the aliases share the parameters' counters)
-        increment_version((self._alias if some is grads else [p for p, g in zip(self._alias, grads) if g is not None]) + self._state)
+        increment_version(self._changed if some is grads else [p for p, g in zip(self._alias, grads) if g is not None] + self._state)
 
     def zero_grad(self):
         for p in self.params:
