@@ -179,6 +179,10 @@ class PairPlan:
         self._ptrs = (base + 8 * n, base + 12 * n, base, base + 16 * n)         # q_ptr, k_ptr, pair_ptr, order
         self._streams = Streams(self.device, [self._dev])
 
+    def __reduce__(self):
+        """A copy (copy.copy, copy.deepcopy, pickle) is a plan of its own: one with this plan's device addresses would outlive the memory behind them."""
+        return PairPlan, (self.q_ptr, self.k_ptr, str(self.device))
+
     @classmethod
     def from_batch(cls, batch, queries: str = "ligand", keys: str = "phore") -> "PairPlan":
         """The plan of an `engine.PackedBatch`: the nodes of one kind attend over the nodes of another (or the same) kind of their complex."""

@@ -460,3 +460,18 @@ def test_a_complex_alone_holds_the_same_bounds(causal, dtype):
     q, k, v, do, b, plan = make([200, 31], [333, 64], 4, 2, 64, dtype, True)
     check(q, k, v, do, b, plan, causal=causal)
     check(q[200:], k[333:], v[333:], do[200:], b[:, 200 * 333:], layers.PairPlan([0, 31], [0, 64]), causal=causal)
+
+
+def test_copies_of_a_plan_have_memory_of_their_own():
+    import copy
+    import pickle
+    q, k, v, _, _, plan = make([5, 40, 7], [9, 70, 3], 2, 2, 16, "f32")
+    out, _ = layers.attention_forward(q, k, v, plan)
+    copies = [copy.copy(plan), copy.deepcopy(plan), pickle.loads(pickle.dumps(plan))]
+    assert len({c._ptrs for c in copies} | {plan._ptrs}) == 4 and all(c._ptrs[2] == c._dev.data_ptr() for c in copies)
+    n = plan._dev.numel()
+    del plan
+    junk = [torch.zeros(n, dtype=torch.int32, device="cuda") for _ in range(16)]
+    for c in copies:
+        assert torch.equal(layers.attention_forward(q, k, v, c)[0], out) and c.n_pairs == 5 * 9 + 40 * 70 + 7 * 3
+    assert len(junk) == 16
