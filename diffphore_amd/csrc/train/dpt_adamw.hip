@@ -10,7 +10,7 @@
 // 8-bit states: m' and v' are formed in 64 bits from the decoded values, the parameter's update uses them unrounded, and the stored codes are the
 // nearest ones.  "Nearest" is decided exactly: a 32-bit root gives the code's position, and where some position of the block lies within its own error of a
 // border between two codes, the block's values are compared with the borders in 64 bits, (c - 1/2)^2 resp. ^4 times the scale (exact, or within 2^-53) -
-// so a code does not depend on the rounding of a root.  This form is bound by instructions as much as by memory: everything that can be is 32 bits.
+// so a code does not depend on the rounding of a root.  This form is bound by instructions as much as by memory (vector units 72 % busy): everything that can be is 32 bits.
 #include "dpt_dev.h"
 
 #include <type_traits>
@@ -74,7 +74,8 @@ struct Values {
   float ms, vs;
 };
 
-// (six waves per SIMD: 540 us for the 120 M parameters against 555 with the registers that the compiler takes for four)
+// (six waves per SIMD: 540 us for the 120 M parameters with 8-bit states against 555 with the registers that the compiler takes for four.  It is a trade: at 80 registers
+// the 8-bit instances spill 13 to 25 of a lane's, among them values of the block that is on its way, which are waited for when they are spilled)
 template <typename P, typename G, int BITS, bool EMA>
 __global__ __launch_bounds__(64 * WAVES, 6) void step_kernel(DptAdamWArgs a, Grads grads) {
   // the step's factors, in 64 bits

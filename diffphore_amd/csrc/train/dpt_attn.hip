@@ -58,7 +58,8 @@ Splits splits_of(const DptAttnArgs* a) {
     return {s, s, s};
   }
   Splits s;
-  // workgroups of one wave: four to a CU; of four waves: one (two, where a kernel is built for that, share it, but each is then the slower)
+  // room is taken as four workgroups of one wave to a CU, or one of four waves (two, where a kernel is built for that, share it, but each is then the slower).  Of the
+  // one-wave ones LDS lets in ten with heads of up to 32 dimensions, four or five of 64, two of 128: four is a middle, not the limit of each
   s.fwd = a->max_nk < 1024 ? 1 : ranges(row_blocks, a->max_nk, small_rows(a) ? 4 * CUS : CUS, 128);   // (shorter walks take less than a join)
   s.q = ranges(row_blocks, a->max_nk, small_rows(a) ? 4 * CUS : CUS, 128);
   s.k = ranges(key_blocks, rows, small_keys(a) ? 4 * CUS : CUS, 128);

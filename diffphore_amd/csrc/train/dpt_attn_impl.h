@@ -109,7 +109,7 @@ __device__ __forceinline__ void zero(f16v* x) {
 // running base and sum per row.  The base follows the row's maximum only when that has moved by more than 2^8 (exp of the difference then still has all its
 // bits, and so has a bf16 of it), so the accumulators are rescaled a few times per row instead of once per tile.
 // Long rows are bound by the matrix units and the exponentials in equal parts (2 x 4096 causal, 16 heads of 128, bf16: 152 us, 903 TFLOP/s; with one wave per SIMD
-// 253 us), single queries by HBM (24 of them against up to 16384 keys: 175 us, 5.2 TB/s), small complexes by latency (40 x (20 x 79) fp32: 11 us).
+// 253 us), single queries by HBM (24 of them against up to 16384 keys: 179 us, 5.1 TB/s), small complexes by latency (40 x (20 x 79) fp32: 11 us).
 template <typename T, int DP, int NW, int BN, bool BIAS, bool VEC>
 __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void fwd_kernel(Dev d) {
   __shared__ __attribute__((aligned(16))) T kt0[BN * DP], vt0[BN * DP], kt1[BN * DP], vt1[BN * DP];
@@ -261,7 +261,9 @@ struct Probs {
 // As the forward pass, with the probabilities formed again from the stored statistics: ds = p (do.v - delta), dq += ds k.  Writes delta = sum_d do o and the
 // rows' factors for the second kernel.  Where a complex's keys are one tile, delta is taken as sum_j p_j do.v_j instead: the stored out is rounded to
 // its type, and with few keys that rounding does not average out.
-// Measured: 225 us for 2 x 4096 causal, 16 heads of 128, bf16 (three products: 917 TFLOP/s); 31 us for 512 complexes of 15 .. 45 x 16 .. 48 with a bias, fp32.
+// Measured: 223 us for 2 x 4096 causal, 16 heads of 128, bf16 (three products: 925 TFLOP/s; at two waves per SIMD 7 registers of a lane are spilled); 31 us for 512
+// complexes of 15 .. 45 x 16 .. 48 with a bias, fp32.  At a head dimension of 128 the instance for short fp32 rows without a bias spills 16 registers, and the
+// one-wave instances for rows that are read element by element spill up to 300 scalar ones.
 template <typename T, int DP, int NW, int BN, bool BIAS, bool VEC>
 __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dq_kernel(Dev d) {
   __shared__ __attribute__((aligned(16))) T kt0[BN * DP], vt0[BN * DP], kt1[BN * DP], vt1[BN * DP];
@@ -401,8 +403,8 @@ __global__ __launch_bounds__(64 * NW, (FAST<T, BIAS> ? 2 : 1)) void dq_kernel(De
 // ---- backward: gradients of the keys and values ---------------------------------------------------------------------------------------------------
 // NW waves x 32 keys; the rows of all heads of the group in tiles of BR, the next one on its way.  Rows down, keys across: the probability and ds tiles
 // are second operands as they stand, dv[d, key] += do[row, d] p[row, key], dk[d, key] += q[row, d] ds[row, key].
-// Measured as above: 402 us (four products: 684 TFLOP/s; at a head dimension of 128 both sums and the wave's keys and values are 230 registers, so one wave per
-// SIMD) and 34 us.
+// Measured as above: 402 us (four products: 684 TFLOP/s; at a head dimension of 128 a lane takes 392 of its 512 registers - both sums, the wave's keys and values and
+// the tiles being worked on -, so one wave per SIMD) and 34 us.
 template <typename T, int DP, int NW, int BR, bool BIAS>
 struct RowTile {
   __attribute__((aligned(16))) T q[BR * DP], g[BR * DP];

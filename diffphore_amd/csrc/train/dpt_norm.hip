@@ -1,14 +1,15 @@
 // dpt_norm.hip - layer norm over the last dimension, forward and backward.
 //
 // Both directions are bound by HBM: x is read once, y written once (backward: x, dy read, dx written).  A row stays in the registers of L lanes
-// (L = 8 .. 512: part of a wave, a wave, or a workgroup), so the statistics are taken in two passes over registers, not over memory:
+// (L = 8 .. 1024: part of a wave, a wave, or a workgroup), so the statistics are taken in two passes over registers, not over memory:
 //   m0 = mean x;  d = x - m0;  c = mean d;  d -= c        (c is what the rounding of m0 left: rows whose entries lie close together need it)
 //   rstd = 1 / sqrt(mean d^2 + eps);  y = d rstd w + b;  mean = m0 + c
 // Backward, with xh = d rstd and g = dy w:  dx = rstd (g - mean g - xh mean(g xh)),  dw = sum_rows dy xh,  db = sum_rows dy.
 // The column sums stay in registers while a group walks over its rows; a workgroup joins its groups in LDS and writes one partial row, a second
 // launch adds the partial rows in a fixed order: no atomics, the same bits every time.
 // Measured: forward 16384 x 4096 bf16 48 us (5.5 TB/s traced, 4.6 from call to call), backward 32749 x 2048 bf16 89 + 8 us (4.5 TB/s for the rows); a copy
-// of 1 GiB runs at 5.0 TB/s.  Backward with three exchanges per row and no row ahead took 188 us.
+// of 1 GiB runs at 5.0 TB/s.  Backward with three exchanges per row and no row ahead took 188 us.  The widest rows pay for their 1024 lanes (128 registers each: up to 6
+// spilled backward, 28 to 32 where a row's length or address does not allow 16-byte reads): 4096 x 16384 bf16 77 forward and 206 us backward, 4096 x 16383 182 and 319.
 #include "dpt_dev.h"
 
 namespace dptn {
