@@ -157,6 +157,7 @@ class AdamW:
     # ---- checkpoints ----------------------------------------------------------------------------------------------------
     def state_dict(self):
         """Copies of the state, with the names and shapes of the tensors that it belongs to (host-synchronising: the step number is read back)."""
+        self._streams.use()
         return {"step": int(self._counter[0].item()), "state_bits": self.state_bits, "names": list(self.names) if self.names is not None else None, "sizes": [tuple(s) for s in self._sizes],
                 **{n: getattr(self, n).clone() if getattr(self, n) is not None else None for n in self._STATE}}
 
@@ -179,6 +180,7 @@ class AdamW:
             raise ValueError("the state belongs to tensors of other shapes, or in another order")
         if names is not None and self.names is not None and list(names) != self.names:
             raise ValueError("the state belongs to tensors of other names, or in another order")
+        self._streams.use()
         for n in self._STATE:
             mine, given = getattr(self, n), state.get(n)
             if (mine is None) != (given is None) or (mine is not None and (mine.shape != given.shape or mine.dtype != given.dtype)):

@@ -440,3 +440,21 @@ def test_every_launch_of_a_long_list_follows_the_formula(dtype, bits):
                 c, s = R.encode(torch.nn.functional.pad(x, (0, -len(x) % 256)), power)
                 lo, hi = opt.first_block[i], opt.first_block[i + 1]
                 assert torch.equal(code[lo * 256:hi * 256].cpu(), c) and torch.allclose(scale[lo:hi].cpu(), s, rtol=2.0 ** -23, atol=0), (i, power)
+
+
+def test_saving_and_loading_on_another_stream_tells_the_allocator():
+    """the copies that state_dict leaves under way read the optimiser's own memory, on whatever stream is current"""
+    params, opt, grads = _setup("bf16", 32, True)
+    opt.step(grads())
+    torch.cuda.synchronize()
+    save, load = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(save):
+        state = opt.state_dict()
+    save.synchronize()
+    _, again, _ = _setup("bf16", 32, True)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(load):
+        again.load_state_dict(state)
+    torch.cuda.synchronize()
+    assert save.cuda_stream in opt._streams._known and load.cuda_stream in again._streams._known
+    assert torch.equal(opt.exp_avg, again.exp_avg) and all(torch.equal(a, b) for a, b in zip(params, again.params))
