@@ -52,8 +52,8 @@ int dpt_layer_norm_bwd(int32_t type, int32_t wtype, int64_t rows, int32_t width,
  * pairs pair_ptr[b] .. pair_ptr[b+1], query-major.  Query head h reads key head h / (heads / kv_heads).
  *   s_ij = scale q_i . k_j + bias[h, pair(b, i, j)];  m_i = max_j s_ij;  l_i = sum_j exp(s_ij - m_i);  out_i = sum_j exp(s_ij - m_i) v_j / l_i
  * causal: key j of a complex is seen by query i iff j <= i + n_keys - n_queries.  A bias of -inf takes the pair out.  A row that sees nothing:
- * out = 0, m = -inf, l = 0, gradients 0.  As in every product of probabilities and values, a NaN or inf in v of a pair that is taken out still
- * reaches the rows of its tile (0 x NaN), and in the backward pass one in q, k or dout. */
+ * out = 0, m = -inf, l = 0, dq = 0.  As in every product of probabilities and values, a NaN or inf in v of a pair that is taken out still reaches
+ * the rows of its tile that see other keys (0 x NaN), and in the backward pass one in q, k or dout.  A row whose scores are NaN has l = NaN. */
 #define DPT_ATTN_MAX_ROWS (0x7fffffff - 1024) /* most rows of q (max_nq times the heads that share a key head, too) and of k */
 
 typedef struct DptAttnArgs {
